@@ -4,6 +4,8 @@
 #   build.sh --profiling [extra hipcc flags]   libvideoitg_hip_prof.so: + research GEMM variants and ablation switches
 #                                              (include/videoitg_hip_profiling.h); loaded by tools/ only, never by the product
 set -euo pipefail
+# no packed fp32 forms (v_pk_add / mul / fma_f32) from hipcc: some of their forms have given wrong results on gfx950 now and then
+NOPK="-Xclang -target-feature -Xclang -packed-fp32-ops"
 HERE="$(cd "$(dirname "${BASH_SOURCE[0]}")" && pwd)"
 HIPCC="${HIPCC:-/opt/rocm/bin/hipcc}"
 SRCS="device gemm gemm256 gemm_mi16 gemm_fp8 attention attention_sp attention_ab elementwise preprocess probe split"
@@ -38,7 +40,7 @@ for f in $SRCS; do
   if [ ! -f "$obj" ] || [ "$src" -nt "$obj" ] || [ "$HERE/common.h" -nt "$obj" ] || [ "$HERE/gemm_common.h" -nt "$obj" ] || [ "$HERE/attn_common.h" -nt "$obj" ] || [ "$HERE/../../include/videoitg_hip.h" -nt "$obj" ]; then
     extra=""
     [ "$f" = "attention_w4" ] && extra="-fno-slp-vectorize"      # its VALU stream is hand-placed in single-issue forms (see st_scale in the file)
-    "$HIPCC" --offload-arch=gfx950 -O3 -std=c++17 -fPIC $DEFS $extra -c "$src" -o "$obj" "$@" &
+    "$HIPCC" --offload-arch=gfx950 -O3 -std=c++17 -fPIC $NOPK $DEFS $extra -c "$src" -o "$obj" "$@" &
     pids+=($!)
     compiled="$compiled $f"
   else
