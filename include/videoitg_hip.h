@@ -291,6 +291,54 @@ int vitg_attention_split(const void* q, const void* k, const void* v, void* o, l
                          int kv_heads, int S, int Sk, int head_dim, long q_bs, long k_bs, long v_bs, long o_bs, int q_rs, int k_rs, int v_rs,
                          int o_rs, int q_hs, int k_hs, int v_hs, int o_hs, float scale, void* stream);
 
+/* ---- Training operators: what a fine-tuning step of the selector needs next to the forward (the reference trains it through autograd of the same modules:
+ * eagle/model/language_model/grounding_qwen2.py:135-169 under train_itg.py).  Gradients never use floating-point atomics: the same call gives the same bits.
+ * Workspaces belong to the call: two calls (or two captured graphs) that may run at the same time need one each.
+ *
+ * vitg_embed_lookup: out[i, :] = scale * table[ids[i], :] (table / out fp32, fp16 or bf16, one rounding); ids outside [0, vocab) - image slots, padding - give
+ *   a zero row.  D, ldt, ldo multiples of 4.  (vitg_embed_gather without a scale, bounds or other types.)  embed_tokens at eagle/model/eagle_archv1.py:310.
+ * vitg_embed_backward: dtable[v, :] = scale * sum over i with ids[i] = v of dout[i, :] for EVERY v < vocab (accumulate = 0: rows without a token are zero), or
+ *   dtable[v, :] += that sum for the rows of the batch only (accumulate = 1).  ids outside the vocabulary contribute nothing.  fp32 sums.  Columns D .. ldt-1
+ *   keep their contents.  workspace: vitg_embed_backward_plan bytes, 16-byte aligned. */
+int vitg_embed_lookup(const long long* ids, long n, const void* table, int table_dtype, long ldt, long vocab, int D, float scale, void* out, int out_dtype,
+                      long ldo, void* stream);
+int vitg_embed_backward_plan(long n, int D, long* workspace_bytes);
+int vitg_embed_backward(const long long* ids, long n, const void* dout, int dout_dtype, long ldd, long vocab, int D, float scale, void* dtable,
+                        int table_dtype, long ldt, int accumulate, void* workspace, long workspace_bytes, void* stream);
+
+/* The gated feed-forward's first half ([3P] Qwen2MLP gate_proj / up_proj / act via grounding_qwen2.py:135): [G | U] = X W^T with the weight rows interleaved
+ * [32 gate | 32 up]... (the layout of VITG_GEMM_SWIGLU), out[M, N/2] = silu(G) * U.
+ * vitg_swiglu: as vitg_gemm(mode = VITG_GEMM_SWIGLU); with gu != NULL it also stores [G | U] rounded to `dtype` in the weight rows' order ([M, N]) for the
+ *   backward pass.  K % 64 == 0, N % 64 == 0, leading dimensions multiples of 8, 16-byte aligned pointers.
+ * vitg_swiglu_backward: from dout = dL/d out and the saved gu: dX = dGU W (type dtype, overwritten) and dW (+)= dGU^T X (type dtype or fp32; accumulate = 1
+ *   adds to what it holds), dGU rounded to dtype once; either of dX / dW may be NULL (then W / X is not read).  workspace: vitg_swiglu_backward_plan bytes,
+ *   16-byte aligned.  M = 0: dW becomes zero (accumulate = 0) or stays. */
+int vitg_swiglu(const void* X, int ldx, const void* W, int ldw, int M, int N, int K, int dtype, void* out, int ldo, void* gu, int ldgu, void* stream);
+int vitg_swiglu_backward_plan(int M, int N, int K, int want_dx, int want_dw, long* workspace_bytes);
+int vitg_swiglu_backward(const void* dout, int lddo, const void* gu, int ldgu, const void* X, int ldx, const void* W, int ldw, int M, int N, int K, int dtype,
+                         void* dX, int lddx, void* dW, int lddw, int dw_dtype, int accumulate, void* workspace, long workspace_bytes, void* stream);
+
+/* The score head and grounding loss (grounding_qwen2.py:148-169) with their gradients.
+ * vitg_pool_score_save: vitg_pool_score on fp32 / fp16 / bf16 rows (row t * tokens_per_frame + j, leading dimension ldh), keeping the frame means
+ *   pooled[frames, ldp] (fp32).
+ * vitg_bce_loss_backward: vitg_bce_loss (out2 = loss, pos_weight) and dlogits = scale * d loss / d logits.
+ * vitg_pool_score_backward: dh[t * tokens_per_frame + j, :] = dlogits[t] / tokens_per_frame * w (fp32 / fp16 / bf16), dw (+)= sum_t dlogits[t] pooled[t, :],
+ *   db (+)= sum_t dlogits[t]; each of dh / dw / db may be NULL; accumulate applies to dw and db. */
+int vitg_pool_score_save(const void* h, int h_dtype, long ldh, int frames, int tokens_per_frame, int D, const float* w, const float* b, float* logits,
+                         float* pooled, long ldp, void* stream);
+int vitg_bce_loss_backward(const float* logits, const float* labels, int n, float scale, float* out2, float* dlogits, void* stream);
+int vitg_pool_score_backward(const float* pooled, long ldp, int frames, int tokens_per_frame, int D, const float* w, const float* dlogits, void* dh,
+                             int dh_dtype, long lddh, float* dw, float* db, int accumulate, void* stream);
+
+/* Global gradient norm over `count` tensors (HOST arrays of device pointers, element counts and dtype codes; contiguous tensors of fp32, fp16, bf16, mixed):
+ * norm[0] = |scale| * sqrt(sum g^2) and, unless outs is NULL, outs[i] = grads[i] * scale * min(1, max_norm / (norm + 1e-6)); outs[i] may be grads[i], and
+ * otherwise overlaps no tensor of the call.  Squares are summed in fp64.  An infinite norm gives factor 0, a NaN norm NaN, as the formula says; max_norm =
+ * infinity scales only.  The addresses travel as kernel arguments: a captured call replays on the same tensors.  workspace: vitg_clip_grad_plan bytes,
+ * 8-byte aligned.  (The reference's Trainer clips with max_grad_norm over all parameters of the model.) */
+int vitg_clip_grad_plan(int count, const long* numel, const int* dtype, long* workspace_bytes);
+int vitg_clip_grad(int count, const void* const* grads, void* const* outs, const long* numel, const int* dtype, float scale, float max_norm, float* norm,
+                   void* workspace, long workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

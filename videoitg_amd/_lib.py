@@ -72,6 +72,18 @@ SIGNATURES = {
     "vitg_rope_split": [_p, _i, _l, _p, _p, _l, _i, _i, _p],
     "vitg_bilinear_pool_split": [_p, _i, _p, _i, _i, _i, _i, _i, _i, _p, _i, _p],
     "vitg_gemm_split16": [_p, _i, _p, _i, _i, _i, _i, _i, _p, _i, _p, _i, _l, _p],
+    # training operators (csrc/train_embed.hip, train_clip.hip, train_head.hip, swiglu.hip)
+    "vitg_embed_lookup": [_p, _l, _p, _i, _l, _l, _i, _f, _p, _i, _l, _p],
+    "vitg_embed_backward_plan": [_l, _i, C.POINTER(C.c_long)],
+    "vitg_embed_backward": [_p, _l, _p, _i, _l, _l, _i, _f, _p, _i, _l, _i, _p, _l, _p],
+    "vitg_swiglu": [_p, _i, _p, _i, _i, _i, _i, _i, _p, _i, _p, _i, _p],
+    "vitg_swiglu_backward_plan": [_i, _i, _i, _i, _i, C.POINTER(C.c_long)],
+    "vitg_swiglu_backward": [_p, _i, _p, _i, _p, _i, _p, _i, _i, _i, _i, _i, _p, _i, _p, _i, _i, _i, _p, _l, _p],
+    "vitg_pool_score_save": [_p, _i, _l, _i, _i, _i, _p, _p, _p, _p, _l, _p],
+    "vitg_bce_loss_backward": [_p, _p, _i, _f, _p, _p, _p],
+    "vitg_pool_score_backward": [_p, _l, _i, _i, _i, _p, _p, _p, _i, _l, _p, _p, _i, _p],
+    "vitg_clip_grad_plan": [_i, C.POINTER(C.c_long), C.POINTER(C.c_int), C.POINTER(C.c_long)],
+    "vitg_clip_grad": [_i, C.POINTER(C.c_void_p), C.POINTER(C.c_void_p), C.POINTER(C.c_long), C.POINTER(C.c_int), _f, _f, _p, _p, _l, _p],
     "vitg_attention_split": [_p, _p, _p, _p, _l, _l, _l, _l, _i, _i, _i, _i, _i, _i, _l, _l, _l, _l, _i, _i, _i, _i, _i, _i, _i, _i, _f, _p],
 }
 

@@ -8,7 +8,7 @@ set -euo pipefail
 NOPK="-Xclang -target-feature -Xclang -packed-fp32-ops"
 HERE="$(cd "$(dirname "${BASH_SOURCE[0]}")" && pwd)"
 HIPCC="${HIPCC:-/opt/rocm/bin/hipcc}"
-SRCS="device gemm gemm256 gemm_mi16 gemm_fp8 attention attention_sp attention_ab elementwise preprocess probe split"
+SRCS="device gemm gemm256 gemm_mi16 gemm_fp8 attention attention_sp attention_ab elementwise preprocess probe split train_embed train_clip train_head swiglu"
 OUT="$HERE/../libvideoitg_hip.so"
 OBJ="$HERE/build"
 DEFS=""
@@ -37,7 +37,7 @@ for f in $SRCS; do
   src="$HERE/$f.hip"; obj="$OBJ/$f.o"
   [ -f "$src" ] || continue
   objs+=("$obj")
-  if [ ! -f "$obj" ] || [ "$src" -nt "$obj" ] || [ "$HERE/common.h" -nt "$obj" ] || [ "$HERE/gemm_common.h" -nt "$obj" ] || [ "$HERE/attn_common.h" -nt "$obj" ] || [ "$HERE/../../include/videoitg_hip.h" -nt "$obj" ]; then
+  if [ ! -f "$obj" ] || [ "$src" -nt "$obj" ] || [ "$HERE/common.h" -nt "$obj" ] || [ "$HERE/gemm_common.h" -nt "$obj" ] || [ "$HERE/attn_common.h" -nt "$obj" ] || [ "$HERE/train_common.h" -nt "$obj" ] || [ "$HERE/../../include/videoitg_hip.h" -nt "$obj" ]; then
     extra=""
     [ "$f" = "attention_w4" ] && extra="-fno-slp-vectorize"      # its VALU stream is hand-placed in single-issue forms (see st_scale in the file)
     "$HIPCC" --offload-arch=gfx950 -O3 -std=c++17 -fPIC $NOPK $DEFS $extra -c "$src" -o "$obj" "$@" &

@@ -40,6 +40,7 @@ struct GemmArgs {
     const float* nrm_colsum;  // consumer: s[n] = sum_k gamma[k] W[n,k] (LayerNorm) or null (RMSNorm: no mean term)
     unsigned* xcd_sync;       // profiling build, gemm_flags bit26: 8 per-XCD arrival counters (128 B apart), zeroed before the launch
     int sk_units, sk_kt;      // stream-K (vitg_gemm_streamk, gemm_mi16.hip): K-tile units per block / K-tiles per output tile; 0 = off
+    void* gu; int ldgu;       // MODE_SWIGLU, SAVE form (vitg_swiglu): the 16-bit pre-activations [gate 32 | up 32]... for the backward pass, [M, N]
     int split_k;              // MODE_F32 only: gridDim.y = split_k blocks share one output tile, block y accumulates its K range and
     long split_stride;        // writes the raw fp32 partial tile to out + y * split_stride floats (vitg_gemm_splitk reduces them)
     // patch embedding with the im2col inside the A-tile loader (vitg_patch_embed16; gemm_mi16.hip PATCH instantiations): A = pixel_values
@@ -314,6 +315,7 @@ bool gemm256_applicable(const GemmArgs& g, int mode);
 int gemm256_pick_cfg(const GemmArgs& g, int mode);                                // the tile shape auto mode takes for this shape (2 / 6 / 9 / 10)
 int gemm256_norm_cols(const GemmArgs& g);                                       // gemm256.hip
 int launch_gemm_mi16_streamk(const GemmArgs& g, int dtype, int blocks, hipStream_t s);   // gemm_mi16.hip: raw fp32 partial tiles of a stream-K partition
+int launch_gemm_mi16_swiglu_save(const GemmArgs& g, int dtype, hipStream_t s);          // gemm_mi16.hip: MODE_SWIGLU that stores its pre-activations too
 int launch_gemm_mi16(const GemmArgs& g, int dtype, int mode, int cfg, hipStream_t s);   // gemm_mi16.hip: the same tiles on v_mfma_f32_16x16x32
 int launch_gemm_w4(const GemmArgs& g, int dtype, int mode, hipStream_t s);      // gemm_w4.hip
 bool gemm_w4_applicable(const GemmArgs& g, int mode);

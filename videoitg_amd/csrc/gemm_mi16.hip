@@ -54,11 +54,14 @@ constexpr int MODE_RES16 = 3;      // internal: MODE_STORE16 with a residual pre
 // SPLIT (round 6, vitg_gemm_split16: the operand-split precision tier, csrc/split.hip): the 16-bit-output epilogues write every value as a PAIR
 // hi = fp16(v) at out[m, n] and lo = fp16(v - hi) at out[m, n + split_off] - the A operand of the next GEMM in K-concatenated form.  Two passes of
 // the same stage loop (the activation is recomputed); the main loop is the same code.  Separate instantiations: the default kernels do not carry it.
-template <typename T, int MODE, int BM, int BN, bool SK = false, int WM = 2, bool PATCH = false, bool SPLIT = false>
+// SAVE (vitg_swiglu with gu): the SwiGLU epilogue also writes the rounded accumulators - the pre-activations [32 gate | 32 up]... in the weight rows'
+// order - for the backward pass; silu(gate) * up itself still comes from the fp32 accumulators.
+template <typename T, int MODE, int BM, int BN, bool SK = false, int WM = 2, bool PATCH = false, bool SPLIT = false, bool SAVE = false>
 __global__ __launch_bounds__(G16_THREADS, 2) void gemm16_kernel(GemmArgs g_) {
     static_assert(!SK || MODE == MODE_F32, "stream-K partials are fp32 tiles");
     static_assert(!SPLIT || MODE == MODE_STORE16 || MODE == MODE_SWIGLU, "split pairs are a 16-bit-output form");
     static_assert(!PATCH || !SK, "the patch loader is not combined with stream-K");
+    static_assert(!SAVE || (MODE == MODE_SWIGLU && !SPLIT), "pre-activations are saved by the plain SwiGLU form");
     typedef typename T16<T>::vec8 vec8;
     GemmArgs g = g_;
     constexpr bool RES16 = MODE == MODE_RES16;
@@ -510,6 +513,33 @@ __global__ __launch_bounds__(G16_THREADS, 2) void gemm16_kernel(GemmArgs g_) {
         else if (g.flags & 0x40000000) stages(AN{}, IY{}, BR{});              // (A/B: bias tested per quad)
         else if (EMODE != MODE_SWIGLU && has_bias) stages(AN{}, IY{}, B1{});
         else stages(AN{}, IY{}, B0{});
+        if constexpr (SAVE) {
+            constexpr int CHG = NT * 2, RBG = NT * 32;                // 16-B chunks and bytes per staged row: 8, 128
+            static_assert((CHG & (CHG - 1)) == 0, "power-of-two chunk count");
+            static_assert((G16_THREADS / 64) * 32 * (RB + RBG) <= 2 * (BM + BN) * 128, "both staging windows of every wave fit the operand ring");
+            char* const stage_gu = smem + (G16_THREADS / 64) * (32 * RB) + wave * (32 * RBG);      // behind the windows of the output rows
+#pragma unroll
+            for (int mp = 0; mp < MT / 2; ++mp) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+                        typename T16<T>::vec4 o;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) o[e] = T16<T>::from_f32(acc[nt][mp * 2 + h][e]);
+                        const int row = h * 16 + r16, c = nt * 2 + (fq >> 1);
+                        *(typename T16<T>::vec4*)(stage_gu + row * RBG + ((c ^ ((row >> 1) & (CHG - 1))) << 4) + (fq & 1) * 8) = o;
+                    }
+                char* const ob = (char*)((T*)g.gu + (size_t)(mw + mp * 32) * g.ldgu + nw);
+#pragma unroll
+                for (int i = 0; i < 32 * CHG / 64; ++i) {
+                    const int idx = i * 64 + lane;
+                    const int row = idx / CHG, c = idx % CHG;
+                    const u32x4 v = *(const u32x4*)(stage_gu + row * RBG + ((c ^ ((row >> 1) & (CHG - 1))) << 4));
+                    if (mw + mp * 32 + row < g.M && nw + c * 8 + 8 <= g.N) *(u32x4*)(ob + (size_t)(unsigned)(row * g.ldgu + c * 8) * 2u) = v;
+                }
+            }
+        }
     }
     if (vb + item_step < item_end) {                     // another tile follows: every wave is done with its staging window
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
@@ -519,14 +549,14 @@ __global__ __launch_bounds__(G16_THREADS, 2) void gemm16_kernel(GemmArgs g_) {
     }   // tile loop
 }
 
-template <typename T, int MODE, int BM, int BN, int WM = 2, bool SPLIT = false>
+template <typename T, int MODE, int BM, int BN, int WM = 2, bool SPLIT = false, bool SAVE = false>
 static int launch16(GemmArgs g, hipStream_t s) {
     constexpr int lds = 2 * (BM + BN) * 128;
     static int done_dev[16] = {0};                       // per device: the attribute belongs to the device's copy of the kernel
     int cur_dev = 0;
     (void)hipGetDevice(&cur_dev);
     if (cur_dev >= 16 || !done_dev[cur_dev]) {
-        (void)hipFuncSetAttribute((const void*)gemm16_kernel<T, MODE, BM, BN, false, WM, false, SPLIT>, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+        (void)hipFuncSetAttribute((const void*)gemm16_kernel<T, MODE, BM, BN, false, WM, false, SPLIT, SAVE>, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
         if (cur_dev < 16) done_dev[cur_dev] = 1;
     }
     g.tiles_m = ceil_div(g.M, BM);
@@ -542,7 +572,7 @@ static int launch16(GemmArgs g, hipStream_t s) {
     // one block per CU walking the tile list when there are at least two tiles per CU (gemm256.hip: "software relaunch")
     const bool loop = nwg >= 2 * cus && !(RESEARCH(gemm_flags) & 0x1000000);
     const int splits = (MODE == MODE_F32 && g.split_k > 1) ? g.split_k : 1;
-    hipLaunchKernelGGL((gemm16_kernel<T, MODE, BM, BN, false, WM, false, SPLIT>), dim3(loop && splits == 1 ? cus : nwg, splits), dim3(G16_THREADS), lds, s, g);
+    hipLaunchKernelGGL((gemm16_kernel<T, MODE, BM, BN, false, WM, false, SPLIT, SAVE>), dim3(loop && splits == 1 ? cus : nwg, splits), dim3(G16_THREADS), lds, s, g);
     return (int)hipGetLastError();
 }
 
@@ -550,6 +580,18 @@ static int launch16(GemmArgs g, hipStream_t s) {
 int launch_gemm_mi16_split(const GemmArgs& g, int mode, hipStream_t s) {
     if (mode == MODE_SWIGLU) return g.M >= 384 ? launch16<f16_t, MODE_SWIGLU, 384, 256, 2, true>(g, s) : launch16<f16_t, MODE_SWIGLU, 256, 256, 2, true>(g, s);
     return g.N >= 384 ? launch16<f16_t, MODE_STORE16, 256, 384, 2, true>(g, s) : launch16<f16_t, MODE_STORE16, 256, 256, 2, true>(g, s);
+}
+
+// SwiGLU keeping its pre-activations: the tile the plain form takes for the shape (gemm256.hip: choose_cfg), 256x256 where that form runs on a smaller one
+int launch_gemm_mi16_swiglu_save(const GemmArgs& g, int dtype, hipStream_t s) {
+    const int cfg = gemm256_applicable(g, MODE_SWIGLU) ? gemm256_pick_cfg(g, MODE_SWIGLU) : 6;
+    auto run = [&](auto t) {
+        typedef decltype(t) T;
+        if (cfg == 10 && g.M >= 384) return launch16<T, MODE_SWIGLU, 384, 256, 2, false, true>(g, s);
+        if (cfg == 12 && g.M > 256) return launch16<T, MODE_SWIGLU, 320, 256, 2, false, true>(g, s);
+        return launch16<T, MODE_SWIGLU, 256, 256, 2, false, true>(g, s);
+    };
+    return dtype == DT_BF16 ? run(bf16_t{}) : run(f16_t{});
 }
 
 #if VITG_PROFILING_BUILD   // stream-K lost its A/B against split-K x2 on the per-rank shapes (profiles/r03_context_parallel.md): profiling library only

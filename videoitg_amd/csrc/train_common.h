@@ -1,0 +1,33 @@
+// Shared between the training operators (train_embed.hip, train_clip.hip, train_head.hip, swiglu.hip): vectors of the three storage types as fp32 values.
+#pragma once
+#include "common.h"
+#include "../../include/videoitg_hip.h"
+
+namespace vitg {
+
+template <typename T> __device__ __forceinline__ float to_f32(T v) { return (float)v; }
+template <typename T> __device__ __forceinline__ T from_f32(float v) { return (T)v; }       // round to nearest even (a plain copy for fp32)
+
+// V consecutive elements of type T <-> fp32 values; p aligned to the vector
+template <typename T, int V> struct Pack { typedef T type __attribute__((ext_vector_type(V))); };
+template <typename T, int V> __device__ __forceinline__ void load_vec(const T* p, float (&v)[V]) {
+    const typename Pack<T, V>::type x = *(const typename Pack<T, V>::type*)p;
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[i] = (float)x[i];
+}
+template <typename T, int V> __device__ __forceinline__ void store_vec(T* p, const float (&v)[V]) {
+    typename Pack<T, V>::type x;
+#pragma unroll
+    for (int i = 0; i < V; ++i) x[i] = (T)v[i];
+    *(typename Pack<T, V>::type*)p = x;
+}
+
+inline bool dtype_ok(int dt) { return dt == DT_BF16 || dt == DT_F16 || dt == DT_F32; }
+inline int dtype_size(int dt) { return dt == DT_F32 ? 4 : 2; }
+inline bool aligned_to(const void* p, int bytes) { return ((uintptr_t)p & (uintptr_t)(bytes - 1)) == 0; }
+inline int launched() { return hipGetLastError() == hipSuccess ? 0 : VITG_ERR_LAUNCH; }
+
+// f(T{}) for the storage type of a dtype code that dtype_ok() has accepted
+template <typename F> inline auto with_dtype(int dt, F f) { return dt == DT_BF16 ? f(bf16_t{}) : dt == DT_F16 ? f(f16_t{}) : f(float{}); }
+
+}  // namespace vitg

@@ -1,0 +1,333 @@
+// Token embedding for training: lookup with a scale, and the gradient of the table.
+//
+//   out[i, :]      = scale * E[ids[i], :]                    ids outside [0, vocab): a zero row (image slots carry -200 in this framework, padding -1)
+//   dE[v, :]  (+)= scale * sum over {i : ids[i] = v} of dout[i, :]
+//
+// The gradient sorts the tokens by id (stable: equal ids keep their order), cuts the sorted list into chunks of `chunk` tokens and lets a block sum the
+// rows of one chunk: a run of equal ids that lies inside one chunk is finished there; a run that crosses chunks leaves fp32 partials, which a second
+// kernel adds in chunk order.  No floating-point atomics: the order of every sum depends on the ids alone, so a repeated call gives the same bits.
+#include "train_common.h"
+
+namespace vitg {
+
+// ---- lookup ------------------------------------------------------------------------------------------------------------------
+template <typename TI, typename TO, int V>
+__global__ void embed_lookup_kernel(const long long* __restrict__ ids, long n, const TI* __restrict__ table, long ldt, long vocab, int cv, float scale,
+                                    TO* __restrict__ out, long ldo) {
+    const long row = (long)blockIdx.x * blockDim.y + threadIdx.y;
+    if (row >= n) return;
+    const long long id = ids[row];
+    const bool known = id >= 0 && id < vocab;
+    for (int c = threadIdx.x; c < cv; c += blockDim.x) {
+        float v[V];
+        if (known) {
+            load_vec<TI, V>(table + id * ldt + (long)c * V, v);
+#pragma unroll
+            for (int e = 0; e < V; ++e) v[e] *= scale;
+        } else {
+#pragma unroll
+            for (int e = 0; e < V; ++e) v[e] = 0.f;
+        }
+        store_vec<TO, V>(out + row * ldo + (long)c * V, v);
+    }
+}
+
+// ---- stable sort of (key, position); key = id, or vocab for a slot without a token (sorts behind every id) ------------------------
+constexpr int SORT_BITS = 9, SORT_BINS = 1 << SORT_BITS, SORT_TILE = 2048, SORT_THREADS = 256;
+
+__device__ __forceinline__ unsigned sort_key(long long id, unsigned vocab) { return id >= 0 && id < (long long)vocab ? (unsigned)id : vocab; }
+
+// one least-significant-digit pass = two launches: digit counts per tile of 2048 keys, then every tile scatters its keys behind the counts of the smaller
+// digits and of the tiles in front of it.  FIRST: the keys are the ids themselves, the positions 0 .. n-1.
+template <bool FIRST>
+__global__ __launch_bounds__(SORT_THREADS) void sort_count_kernel(const long long* __restrict__ ids, const unsigned* __restrict__ key_in, long n, unsigned vocab,
+                                                                  int shift, unsigned* __restrict__ counts) {
+    __shared__ unsigned bins[SORT_BINS];
+    for (int b = threadIdx.x; b < SORT_BINS; b += SORT_THREADS) bins[b] = 0;
+    __syncthreads();
+    const long base = (long)blockIdx.x * SORT_TILE;
+    for (int k = threadIdx.x; k < SORT_TILE; k += SORT_THREADS) {
+        const long i = base + k;
+        if (i < n) atomicAdd(&bins[((FIRST ? sort_key(ids[i], vocab) : key_in[i]) >> shift) & (SORT_BINS - 1)], 1u);
+    }
+    __syncthreads();
+    for (int b = threadIdx.x; b < SORT_BINS; b += SORT_THREADS) counts[(size_t)blockIdx.x * SORT_BINS + b] = bins[b];
+}
+
+template <bool FIRST>
+__global__ __launch_bounds__(SORT_THREADS) void sort_scatter_kernel(const long long* __restrict__ ids, const unsigned* __restrict__ key_in,
+                                                                    const unsigned* __restrict__ pos_in, long n, unsigned vocab, int shift, int tiles,
+                                                                    const unsigned* __restrict__ counts, unsigned* __restrict__ key_out, unsigned* __restrict__ pos_out) {
+    constexpr int WAVES = SORT_THREADS / 64, ROUNDS = SORT_TILE / SORT_THREADS, BPT = SORT_BINS / SORT_THREADS;
+    __shared__ unsigned next[WAVES][SORT_BINS];          // next free slot of a digit for one wave's keys
+    __shared__ unsigned wave_total[WAVES];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    // thread t owns digits BPT t ..: keys with that digit in all tiles, and in the tiles in front of this one
+    unsigned total[BPT], before[BPT], mine = 0;
+#pragma unroll
+    for (int d = 0; d < BPT; ++d) {
+        total[d] = before[d] = 0;
+        for (int t = 0; t < tiles; ++t) {
+            const unsigned c = counts[(size_t)t * SORT_BINS + tid * BPT + d];
+            total[d] += c;
+            if (t < (int)blockIdx.x) before[d] += c;
+        }
+        mine += total[d];
+    }
+    unsigned scan = mine;                                // exclusive prefix over the threads (= over the digits)
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) { const unsigned up = __shfl_up(scan, o, 64); if (lane >= o) scan += up; }
+    if (lane == 63) wave_total[wave] = scan;
+    for (int b = tid; b < WAVES * SORT_BINS; b += SORT_THREADS) (&next[0][0])[b] = 0;
+    __syncthreads();
+    unsigned first = scan - mine;
+    for (int w = 0; w < wave; ++w) first += wave_total[w];
+    // this wave's keys: 64 consecutive ones per round, ROUNDS rounds; counts per digit
+    unsigned key[ROUNDS], pos[ROUNDS];
+    const long base = (long)blockIdx.x * SORT_TILE + wave * (ROUNDS * 64) + lane;
+#pragma unroll
+    for (int r = 0; r < ROUNDS; ++r) {
+        const long i = base + r * 64;
+        key[r] = 0; pos[r] = 0;
+        if (i < n) {
+            key[r] = FIRST ? sort_key(ids[i], vocab) : key_in[i];
+            pos[r] = FIRST ? (unsigned)i : pos_in[i];
+            atomicAdd(&next[wave][(key[r] >> shift) & (SORT_BINS - 1)], 1u);
+        }
+    }
+    __syncthreads();
+    // counts -> first slot: digits below, tiles in front, waves in front
+#pragma unroll
+    for (int d = 0; d < BPT; ++d) {
+        unsigned at = first + before[d];
+        first += total[d];
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) { const unsigned c = next[w][tid * BPT + d]; next[w][tid * BPT + d] = at; at += c; }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < ROUNDS; ++r) {
+        const bool live = base + r * 64 < n;
+        const unsigned digit = (key[r] >> shift) & (SORT_BINS - 1);
+        unsigned long long same = __ballot(live);        // lanes of this round with the same digit
+#pragma unroll
+        for (int b = 0; b < SORT_BITS; ++b) {
+            const unsigned long long m = __ballot((digit >> b) & 1u);
+            same &= ((digit >> b) & 1u) ? m : ~m;
+        }
+        const unsigned rank = __popcll(same & ((1ull << lane) - 1ull));
+        // (one wave's LDS operations complete in order: every lane has read the slot before the first lane of its digit moves it on)
+        volatile unsigned* const slot = &next[wave][digit];
+        unsigned at = 0;
+        if (live) at = *slot + rank;
+        __builtin_amdgcn_wave_barrier();
+        if (live && rank == 0) *slot = at + __popcll(same);
+        __builtin_amdgcn_wave_barrier();
+        if (live) { key_out[at] = key[r]; pos_out[at] = pos[r]; }
+    }
+}
+
+// ---- the sums ----------------------------------------------------------------------------------------------------------------------
+// zero rows of the dense form (accumulate = 0): the rows of the batch's tokens are overwritten by the kernels below
+template <int V, typename T>
+__global__ __launch_bounds__(256) void zero_rows_kernel(T* __restrict__ table, long ldt, long rows, int cv) {
+    float z[V];
+#pragma unroll
+    for (int e = 0; e < V; ++e) z[e] = 0.f;
+    for (long r = blockIdx.x; r < rows; r += gridDim.x)
+        for (int c = threadIdx.x; c < cv; c += 256) store_vec<T, V>(table + r * ldt + (long)c * V, z);
+}
+
+template <typename TT, int V>
+__device__ __forceinline__ void finish_row(TT* __restrict__ row, int accumulate, float scale, const float (&acc)[V]) {
+    float v[V];
+    if (accumulate) load_vec<TT, V>(row, v);
+#pragma unroll
+    for (int e = 0; e < V; ++e) v[e] = accumulate ? v[e] + scale * acc[e] : scale * acc[e];
+    store_vec<TT, V>(row, v);
+}
+
+// partials: [chunk][2][cv * V] fp32 - slot 0: a run that began in an earlier chunk, slot 1: a run that begins here and goes on behind it
+template <typename TD, typename TT, int V>
+__global__ __launch_bounds__(256) void embed_grad_kernel(const unsigned* __restrict__ key, const unsigned* __restrict__ pos, long n, unsigned vocab, int chunk,
+                                                         const TD* __restrict__ dout, long ldd, int cv, float scale, TT* __restrict__ table, long ldt,
+                                                         int accumulate, float* __restrict__ partial) {
+    const int c = blockIdx.y * 256 + threadIdx.x;
+    if (c >= cv) return;
+    const long e0 = (long)blockIdx.x * chunk, e1 = min(e0 + chunk, n);
+    unsigned run = key[e0];
+    if (run >= vocab) return;                            // nothing but slots without a token from here on
+    bool began = e0 == 0 || key[e0 - 1] != run;
+    float acc[V];
+#pragma unroll
+    for (int e = 0; e < V; ++e) acc[e] = 0.f;
+    for (long e = e0; e < e1; ++e) {
+        float v[V];
+        load_vec<TD, V>(dout + (long)pos[e] * ldd + (long)c * V, v);
+#pragma unroll
+        for (int k = 0; k < V; ++k) acc[k] += v[k];
+        const unsigned after = e + 1 < n ? key[e + 1] : vocab;
+        if (after != run) {                              // the run ends with this token
+            if (began) finish_row<TT, V>(table + (long)run * ldt + (long)c * V, accumulate, scale, acc);
+            else store_vec<float, V>(partial + ((size_t)blockIdx.x * 2) * ((size_t)cv * V) + (size_t)c * V, acc);
+            if (after >= vocab) return;
+            run = after;
+            began = true;
+#pragma unroll
+            for (int k = 0; k < V; ++k) acc[k] = 0.f;
+            if (e + 1 == e1) return;                     // the next run starts the next chunk
+        }
+    }
+    // the run goes on in the next chunk
+    store_vec<float, V>(partial + ((size_t)blockIdx.x * 2 + (began ? 1 : 0)) * ((size_t)cv * V) + (size_t)c * V, acc);
+}
+
+// runs across chunks: the block of the chunk in which a run begins adds its partials in chunk order - the waves take consecutive parts of the list,
+// their sums join through LDS in wave order
+constexpr int JOIN_WAVES = 8;
+template <typename TT>
+__global__ __launch_bounds__(JOIN_WAVES * 64) void embed_join_kernel(const unsigned* __restrict__ key, long n, unsigned vocab, int chunk, int D, float scale,
+                                                                     TT* __restrict__ table, long ldt, int accumulate, const float* __restrict__ partial) {
+    constexpr int V = 4;
+    __shared__ float part[JOIN_WAVES][64 * V];
+    const long b = blockIdx.x, chunks = (n + chunk - 1) / chunk;
+    if (b + 1 >= chunks) return;
+    const unsigned run = key[(b + 1) * chunk - 1];
+    if (run >= vocab || key[(b + 1) * chunk] != run || (b > 0 && key[b * chunk - 1] == run)) return;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    long last = b + 1;                                   // last chunk that holds a part of the run
+    for (;;) {
+        const long j = last + 1 + lane;
+        const unsigned long long in = __ballot(j < chunks && key[min(j, chunks - 1) * chunk] == run);
+        const int more = in == ~0ull ? 64 : __ffsll((unsigned long long)~in) - 1;
+        last += more;
+        if (more < 64) break;
+    }
+    const int c = (blockIdx.y * 64 + lane) * V;
+    const long items = last - b + 1, per = (items + JOIN_WAVES - 1) / JOIN_WAVES;
+    float acc[V] = {0.f, 0.f, 0.f, 0.f};
+    if (c < D)
+        for (long i = wave * per; i < min((wave + 1) * per, items); ++i) {
+            float v[V];
+            load_vec<float, V>(partial + ((size_t)(b + i) * 2 + (i == 0 ? 1 : 0)) * (size_t)D + c, v);
+#pragma unroll
+            for (int k = 0; k < V; ++k) acc[k] += v[k];
+        }
+    store_vec<float, V>(&part[wave][lane * V], acc);
+    __syncthreads();
+    if (wave == 0 && c < D) {
+        for (int w = 1; w < JOIN_WAVES; ++w)
+#pragma unroll
+            for (int k = 0; k < V; ++k) acc[k] += part[w][lane * V + k];
+        finish_row<TT, V>(table + (long)run * ldt + c, accumulate, scale, acc);
+    }
+}
+
+// tokens per chunk
+static int embed_chunk(long n) { return n >= 32768 ? 32 : 16; }
+static size_t round256(size_t b) { return (b + 255) & ~(size_t)255; }
+
+struct EmbedWorkspace { size_t key[2], pos[2], counts, partial, bytes; int tiles, chunk; long chunks; };
+static EmbedWorkspace embed_workspace(long n, int D) {
+    EmbedWorkspace w;
+    w.tiles = (int)((n + SORT_TILE - 1) / SORT_TILE);
+    w.chunk = embed_chunk(n);
+    w.chunks = (n + w.chunk - 1) / w.chunk;
+    size_t at = 0;
+    for (int i = 0; i < 2; ++i) { w.key[i] = at; at += round256((size_t)n * 4); w.pos[i] = at; at += round256((size_t)n * 4); }
+    w.counts = at; at += round256((size_t)w.tiles * SORT_BINS * 4);
+    w.partial = at; at += round256((size_t)w.chunks * 2 * D * 4);
+    w.bytes = at;
+    return w;
+}
+
+}  // namespace vitg
+
+using namespace vitg;
+
+extern "C" int vitg_embed_lookup(const long long* ids, long n, const void* table, int table_dtype, long ldt, long vocab, int D, float scale, void* out,
+                                 int out_dtype, long ldo, void* stream) {
+    if (n <= 0) return 0;
+    if (!ids || !table || !out) return VITG_ERR_ARG;
+    if (!dtype_ok(table_dtype) || !dtype_ok(out_dtype)) return VITG_ERR_DTYPE;
+    if (vocab <= 0 || D <= 0 || n >= (1l << 31) || ldt < D || ldo < D) return VITG_ERR_SHAPE;
+    if (D % 4 || ldt % 4 || ldo % 4 || !aligned_to(table, 4 * dtype_size(table_dtype)) || !aligned_to(out, 4 * dtype_size(out_dtype))) return VITG_ERR_ALIGN;
+    const bool wide = D % 8 == 0 && ldt % 8 == 0 && ldo % 8 == 0 && aligned_to(table, 16) && aligned_to(out, 16);
+    const int cv = D / (wide ? 8 : 4);
+    const int tx = cv >= 512 ? 512 : (cv + 63) / 64 * 64, ty = tx >= 256 ? 1 : 256 / tx;
+    const dim3 grid((unsigned)((n + ty - 1) / ty)), block(tx, ty);
+    with_dtype(table_dtype, [&](auto ti) {
+        typedef decltype(ti) TI;
+        with_dtype(out_dtype, [&](auto to) {
+            typedef decltype(to) TO;
+            if (wide) hipLaunchKernelGGL((embed_lookup_kernel<TI, TO, 8>), grid, block, 0, (hipStream_t)stream, ids, n, (const TI*)table, ldt, vocab, cv, scale, (TO*)out, ldo);
+            else hipLaunchKernelGGL((embed_lookup_kernel<TI, TO, 4>), grid, block, 0, (hipStream_t)stream, ids, n, (const TI*)table, ldt, vocab, cv, scale, (TO*)out, ldo);
+        });
+    });
+    return launched();
+}
+
+extern "C" int vitg_embed_backward_plan(long n, int D, long* workspace_bytes) {
+    if (!workspace_bytes) return VITG_ERR_ARG;
+    if (n < 0 || n >= (1l << 31) || D <= 0) return VITG_ERR_SHAPE;
+    *workspace_bytes = n ? (long)embed_workspace(n, D).bytes : 0;
+    return 0;
+}
+
+extern "C" int vitg_embed_backward(const long long* ids, long n, const void* dout, int dout_dtype, long ldd, long vocab, int D, float scale, void* dtable,
+                                   int table_dtype, long ldt, int accumulate, void* workspace, long workspace_bytes, void* stream) {
+    if (n < 0 || vocab <= 0 || D <= 0 || n >= (1l << 31) || vocab >= (1l << 31) - 1 || ldt < D) return VITG_ERR_SHAPE;
+    if (!dtable || (n && (!ids || !dout || !workspace))) return VITG_ERR_ARG;
+    if (!dtype_ok(table_dtype) || !dtype_ok(dout_dtype)) return VITG_ERR_DTYPE;
+    if (n && ldd < D) return VITG_ERR_SHAPE;
+    if (D % 4 || ldt % 4 || (n && ldd % 4) || !aligned_to(dtable, 4 * dtype_size(table_dtype)) || (n && !aligned_to(dout, 4 * dtype_size(dout_dtype)))) return VITG_ERR_ALIGN;
+    const EmbedWorkspace w = n ? embed_workspace(n, D) : EmbedWorkspace{};
+    if (n && (workspace_bytes < (long)w.bytes || !aligned_to(workspace, 16))) return VITG_ERR_ARG;
+    hipStream_t s = (hipStream_t)stream;
+    if (!accumulate) {
+        const bool wide = D % 8 == 0 && ldt % 8 == 0 && aligned_to(dtable, 16);
+        const unsigned grid = (unsigned)(vocab < 8192 ? vocab : 8192);
+        with_dtype(table_dtype, [&](auto tt) {
+            typedef decltype(tt) TT;
+            if (wide) hipLaunchKernelGGL((zero_rows_kernel<8, TT>), dim3(grid), dim3(256), 0, s, (TT*)dtable, ldt, vocab, D / 8);
+            else hipLaunchKernelGGL((zero_rows_kernel<4, TT>), dim3(grid), dim3(256), 0, s, (TT*)dtable, ldt, vocab, D / 4);
+        });
+    }
+    if (n == 0) return launched();
+    char* const base = (char*)workspace;
+    unsigned *key[2], *pos[2], *counts = (unsigned*)(base + w.counts);
+    for (int i = 0; i < 2; ++i) { key[i] = (unsigned*)(base + w.key[i]); pos[i] = (unsigned*)(base + w.pos[i]); }
+    float* const partial = (float*)(base + w.partial);
+    int bits = 1;
+    while ((vocab >> bits) != 0) ++bits;                 // keys 0 .. vocab
+    const unsigned v = (unsigned)vocab;
+    int cur = 0;
+    for (int shift = 0, pass = 0; shift < bits; shift += SORT_BITS, ++pass) {
+        const int to = cur ^ 1;
+        if (pass == 0) {
+            hipLaunchKernelGGL(sort_count_kernel<true>, dim3(w.tiles), dim3(SORT_THREADS), 0, s, ids, nullptr, n, v, shift, counts);
+            hipLaunchKernelGGL(sort_scatter_kernel<true>, dim3(w.tiles), dim3(SORT_THREADS), 0, s, ids, nullptr, nullptr, n, v, shift, w.tiles, counts, key[to], pos[to]);
+        } else {
+            hipLaunchKernelGGL(sort_count_kernel<false>, dim3(w.tiles), dim3(SORT_THREADS), 0, s, nullptr, key[cur], n, v, shift, counts);
+            hipLaunchKernelGGL(sort_scatter_kernel<false>, dim3(w.tiles), dim3(SORT_THREADS), 0, s, nullptr, key[cur], pos[cur], n, v, shift, w.tiles, counts, key[to], pos[to]);
+        }
+        cur = to;
+    }
+    const bool wide = D % 8 == 0 && ldt % 8 == 0 && ldd % 8 == 0 && aligned_to(dtable, 16) && aligned_to(dout, 16);
+    const int cv = D / (wide ? 8 : 4);
+    with_dtype(dout_dtype, [&](auto td) {
+        typedef decltype(td) TD;
+        with_dtype(table_dtype, [&](auto tt) {
+            typedef decltype(tt) TT;
+            const dim3 grid((unsigned)w.chunks, ceil_div(cv, 256));
+            if (wide) hipLaunchKernelGGL((embed_grad_kernel<TD, TT, 8>), grid, dim3(256), 0, s, key[cur], pos[cur], n, v, w.chunk, (const TD*)dout, ldd, cv, scale, (TT*)dtable, ldt, accumulate, partial);
+            else hipLaunchKernelGGL((embed_grad_kernel<TD, TT, 4>), grid, dim3(256), 0, s, key[cur], pos[cur], n, v, w.chunk, (const TD*)dout, ldd, cv, scale, (TT*)dtable, ldt, accumulate, partial);
+        });
+    });
+    if (w.chunks > 1)
+        with_dtype(table_dtype, [&](auto tt) {
+            typedef decltype(tt) TT;
+            hipLaunchKernelGGL((embed_join_kernel<TT>), dim3((unsigned)w.chunks, ceil_div(D, 256)), dim3(JOIN_WAVES * 64), 0, s, key[cur], n, v, w.chunk, D, scale, (TT*)dtable, ldt, accumulate, partial);
+        });
+    return launched();
+}

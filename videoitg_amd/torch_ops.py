@@ -17,7 +17,8 @@ aliasing behaviour.
 ``SelectorEngine`` launches through this module (``videoitg_amd.engine.K``); ``videoitg_amd.ops`` stays the raw binding.
 Names are the build's choice: patchify, gemm, layernorm, rmsnorm, rope_, attention, bilinear_pool,
 gather_rows, embed_gather, pool_score, rank, preprocess_u8, bce_loss, quant_rows_fp8, norm_quant_fp8, gemm_fp8, gemm_fp8_mx,
-gemm_res16 / layernorm16 / bilinear_pool16 (the tower's 16-bit residual stream).
+gemm_res16 / layernorm16 / bilinear_pool16 (the tower's 16-bit residual stream),
+embed_lookup / embed_backward, swiglu / swiglu_backward, pool_score_save / bce_loss_backward / pool_score_backward, grad_norm / clip_grad_norm(_) (training).
 """
 from __future__ import annotations
 
@@ -179,6 +180,41 @@ _def("gemm_fp8_mx(Tensor a8, Tensor w8, Tensor sw, Tensor(a!) out, int out_dtype
          (_raw.gemm_fp8_mx(a8, w8, sw, out, out_dtype=_DT[out_dtype], sa=sa, a_mx=a_mx, o_mx=o_mx, n=n, bias=bias, act=act, res=res, m=m,
                            swiglu=swiglu), None)[1],
      lambda *a, **k: None)
+
+# ---- training operators --------------------------------------------------------------------------------------------------------
+_def("embed_lookup(Tensor ids, Tensor table, Tensor(a!) out, float scale=1.0) -> ()",
+     lambda ids, table, out, scale=1.0: (_raw.embed_lookup(ids, table, out, scale=scale), None)[1], lambda *a, **k: None)
+_def("embed_backward(Tensor ids, Tensor dout, Tensor(a!) dtable, float scale=1.0, bool accumulate=False, Tensor(b!)? workspace=None) -> ()",
+     lambda ids, dout, dtable, scale=1.0, accumulate=False, workspace=None:
+         (_raw.embed_backward(ids, dout, dtable, scale=scale, accumulate=accumulate, workspace=workspace), None)[1],
+     lambda *a, **k: None)
+_def("swiglu(Tensor x, Tensor w, Tensor(a!) out, Tensor(b!)? gu=None) -> ()",
+     lambda x, w, out, gu=None: (_raw.swiglu(x, w, out, gu=gu), None)[1], lambda *a, **k: None)
+_def("swiglu_backward(Tensor dout, Tensor gu, Tensor x, Tensor w, Tensor(a!)? dx=None, Tensor(b!)? dw=None, bool accumulate=False, "
+     "Tensor(c!)? workspace=None) -> ()",
+     lambda dout, gu, x, w, dx=None, dw=None, accumulate=False, workspace=None:
+         _raw.swiglu_backward(dout, gu, x, w, dx=dx, dw=dw, accumulate=accumulate, workspace=workspace),
+     lambda *a, **k: None)
+_def("pool_score_save(Tensor h, int frames, int tokens_per_frame, int d, Tensor w, Tensor b, Tensor(a!) logits, Tensor(b!) pooled) -> ()",
+     lambda h, frames, tokens_per_frame, d, w, b, logits, pooled: (_raw.pool_score_save(h, frames, tokens_per_frame, d, w, b, logits, pooled), None)[1],
+     lambda *a, **k: None)
+_def("bce_loss_backward(Tensor logits, Tensor labels, float scale=1.0) -> (Tensor, Tensor, Tensor)",
+     lambda logits, labels, scale=1.0: _raw.bce_loss_backward(logits, labels, scale=scale),
+     lambda logits, labels, scale=1.0: (logits.new_empty(()), logits.new_empty(()), logits.new_empty(logits.shape)))
+_def("pool_score_backward(Tensor pooled, int frames, int tokens_per_frame, int d, Tensor w, Tensor dlogits, Tensor(a!)? dh=None, Tensor(b!)? dw=None, "
+     "Tensor(c!)? db=None, bool accumulate=False) -> ()",
+     lambda pooled, frames, tokens_per_frame, d, w, dlogits, dh=None, dw=None, db=None, accumulate=False:
+         _raw.pool_score_backward(pooled, frames, tokens_per_frame, d, w, dlogits, dh, dw=dw, db=db, accumulate=accumulate),
+     lambda *a, **k: None)
+_def("grad_norm(Tensor[] grads, float scale=1.0) -> Tensor",
+     lambda grads, scale=1.0: _raw.clip_grad_norm(grads, None, scale=scale),
+     lambda grads, scale=1.0: grads[0].new_empty(1, dtype=torch.float32))
+_def("clip_grad_norm(Tensor[] grads, Tensor(a!)[] outs, float max_norm, float scale=1.0) -> Tensor",
+     lambda grads, outs, max_norm, scale=1.0: _raw.clip_grad_norm(grads, max_norm, outs=outs, scale=scale),
+     lambda grads, outs, max_norm, scale=1.0: grads[0].new_empty(1, dtype=torch.float32))
+_def("clip_grad_norm_(Tensor(a!)[] grads, float max_norm, float scale=1.0) -> Tensor",
+     lambda grads, max_norm, scale=1.0: _raw.clip_grad_norm(grads, max_norm, scale=scale),
+     lambda grads, max_norm, scale=1.0: grads[0].new_empty(1, dtype=torch.float32))
 
 # ---- call-compatible namespace for the engine (same signatures as videoitg_amd.ops) ------------------------------------
 _ops = torch.ops.videoitg
@@ -369,9 +405,52 @@ class _Namespace:
     def preprocess_u8(frames, size, out_dtype=torch.float32):
         return _ops.preprocess_u8(frames, size, _CODE[out_dtype])
 
+    embed_backward_plan = staticmethod(_raw.embed_backward_plan)
+    swiglu_backward_plan = staticmethod(_raw.swiglu_backward_plan)
+
+    @staticmethod
+    def embed_lookup(ids, table, out, *, scale=1.0):
+        _ops.embed_lookup(ids, table, out, scale)
+        return out
+
+    @staticmethod
+    def embed_backward(ids, dout, dtable, *, scale=1.0, accumulate=False, workspace=None):
+        _ops.embed_backward(ids, dout, dtable, scale, accumulate, workspace)
+        return dtable
+
+    @staticmethod
+    def swiglu(x, w, out, *, gu=None):
+        _ops.swiglu(x, w, out, gu)
+        return out
+
+    @staticmethod
+    def swiglu_backward(dout, gu, x, w, *, dx=None, dw=None, accumulate=False, workspace=None):
+        _ops.swiglu_backward(dout, gu, x, w, dx, dw, accumulate, workspace)
+
+    @staticmethod
+    def pool_score_save(h, frames, tokens_per_frame, d, w, b, logits, pooled):
+        _ops.pool_score_save(h, frames, tokens_per_frame, d, w, b, logits, pooled)
+        return logits
+
+    @staticmethod
+    def bce_loss_backward(logits, labels, *, scale=1.0):
+        return _ops.bce_loss_backward(logits, labels, scale)
+
+    @staticmethod
+    def pool_score_backward(pooled, frames, tokens_per_frame, d, w, dlogits, dh=None, *, dw=None, db=None, accumulate=False):
+        _ops.pool_score_backward(pooled, frames, tokens_per_frame, d, w, dlogits, dh, dw, db, accumulate)
+
+    @staticmethod
+    def clip_grad_norm(grads, max_norm, *, outs=None, scale=1.0):
+        if max_norm is None:
+            return _ops.grad_norm(grads, scale)
+        return _ops.clip_grad_norm_(grads, max_norm, scale) if outs is None else _ops.clip_grad_norm(grads, outs, max_norm, scale)
+
 
 K = _Namespace()
 OP_NAMES: List[str] = ["patchify", "gemm", "gemm_splitk", "gemm_splitk16", "layernorm", "rmsnorm", "rope_", "attention", "bilinear_pool", "gather_rows",
                        "embed_gather", "pool_score", "rank", "bce_loss", "preprocess_u8", "quant_rows_fp8", "norm_quant_fp8", "gemm_fp8", "gemm_fp8_mx",
                        "gemm_res16", "layernorm16", "bilinear_pool16", "patch_embed16", "norm_quant_fp8_16", "gemm_fp8_res16",
-                       "norm_split", "rope_split_", "bilinear_pool_split", "gemm_split16", "attention_split"] + (["gemm_streamk"] if _raw._lib.PROFILING else [])
+                       "norm_split", "rope_split_", "bilinear_pool_split", "gemm_split16", "attention_split",
+                       "embed_lookup", "embed_backward", "swiglu", "swiglu_backward", "pool_score_save", "bce_loss_backward", "pool_score_backward",
+                       "grad_norm", "clip_grad_norm", "clip_grad_norm_"] + (["gemm_streamk"] if _raw._lib.PROFILING else [])
