@@ -126,7 +126,7 @@ def test_embed_backward_types_and_strides(ops, dout_dtype, table_dtype, accumula
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("n,vocab,kind", [(70001, 300000, "mixed"), (40000, 3, "spread"), (33000, 152064, "one_id"), (65536, 2 ** 27 - 3, "spread")])
+@pytest.mark.parametrize("n,vocab,kind", [(15360, 9000, "mixed"), (15361, 9000, "mixed"), (15361, 400, "none"), (70001, 300000, "mixed"), (40000, 3, "spread"), (33000, 152064, "one_id"), (65536, 2 ** 27 - 3, "spread")])
 def test_embed_backward_long_lists(ops, n, vocab, kind):
     """several digits per key, many sort tiles, runs over hundreds of chunks; the touched rows of a large vocabulary only"""
     d = 8
@@ -140,6 +140,9 @@ def test_embed_backward_long_lists(ops, n, vocab, kind):
     table = torch.zeros(vocab, d, device="cuda")
     ops.embed_backward(ids.cuda(), dout.cuda(), table, accumulate=True)
     assert int((table != 0).any(1).sum()) == len(token)
+    dense = torch.full((vocab, d), 5.0, dtype=F32, device="cuda") if vocab < 10 ** 6 else None
+    if dense is not None:
+        assert torch.equal(ops.embed_backward(ids.cuda(), dout.cuda(), dense), table)
     # a row's terms are added in chunks of 32 and then chunk by chunk, in eight parts: far fewer roundings than n; the bound counts 32 + n / 256 + 8
     within(table[token.cuda()], want, (48 + n / 256) * U32 * mass)
 
@@ -204,7 +207,7 @@ def ffn_grads(dout, gu, x, w):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [BF16, F16])
-@pytest.mark.parametrize("m,k,n", FFN_SHAPES + [(129, 1024, 4096), (300, 256, 8192)])
+@pytest.mark.parametrize("m,k,n", FFN_SHAPES + [(129, 1024, 4096), (300, 256, 8192), (33, 576, 1024), (2100, 64, 128), (3000, 320, 192), (5000, 512, 64)])
 @pytest.mark.parametrize("dw_kind", ["same", "same_add", "fp32", "fp32_add"])
 def test_swiglu_backward(ops, dtype, m, k, n, dw_kind):
     x, w = randn(m, k, dtype=dtype), randn(n, k, dtype=dtype, scale=k ** -0.5)
@@ -565,9 +568,15 @@ def test_head_and_clip_entries_refuse(lib):
     assert lib.vitg_clip_grad_plan(-1, one, f32, C.byref(need)) == SHAPE and lib.vitg_clip_grad_plan(1, (C.c_long * 1)(-1), f32, C.byref(need)) == SHAPE
     assert lib.vitg_clip_grad_plan(1, one, (C.c_int * 1)(9), C.byref(need)) == DTYPE
 
-    def clip(count=1, g=ptr, o=ptr, numel=one, dt=f32, max_norm=1.0, norm=P, ws=P, bytes_=64):
+    far = C.c_void_p(1 << 20)
+
+    def clip(count=1, g=ptr, o=ptr, numel=one, dt=f32, max_norm=1.0, norm=C.c_void_p(1 << 16), ws=far, bytes_=64):
         return lib.vitg_clip_grad(count, g, o, numel, dt, 1.0, max_norm, norm, ws, bytes_, NUL)
     assert clip(g=nul) == ARG and clip(o=nul) == ARG and clip(norm=NUL) == ARG and clip(ws=NUL) == ARG and clip(bytes_=4) == ARG and clip(max_norm=-1.0) == ARG
+    both, five, kinds = C.c_void_p * 2, (C.c_long * 2)(5, 5), (C.c_int * 2)(2, 2)
+    for g, o in (((4096, 4096), (4096, 4096)), ((4096, 4112), (4096, 4112)), ((4096, 8192), (8192, 12288)), ((4096, 8192), (12288, 12300)), ((4096, 8192), (4100, 8192))):
+        assert clip(count=2, g=both(*g), o=both(*o), numel=five, dt=kinds) == ARG, (g, o)        # two tensors on one byte that is written
+    assert clip(norm=C.c_void_p(4100)) == ARG and clip(ws=P) == ARG
     assert clip(max_norm=float("nan")) == ARG and clip(g=odd) == ALIGN and clip(dt=(C.c_int * 1)(3)) == DTYPE and clip(count=-1) == SHAPE
 
 

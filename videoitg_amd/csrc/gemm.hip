@@ -132,6 +132,14 @@ __global__ __launch_bounds__(GEMM_THREADS, 2) void gemm128_kernel(GemmArgs g) {
                     v[e] = T16<T>::from_f32(silu_f(gt) * up);
                 }
                 *(typename T16<T>::vec4*)(out + (size_t)m * g.ldo + no) = v;
+                if (g.gu) {                                      // vitg_swiglu: the pre-activations, rounded, for the backward pass
+                    typename T16<T>::vec4 pg, pu;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) { pg[e] = T16<T>::from_f32(acc[0][mt][q4 * 4 + e]); pu[e] = T16<T>::from_f32(acc[1][mt][q4 * 4 + e]); }
+                    T* const gu = (T*)g.gu + (size_t)m * g.ldgu + nn;
+                    *(typename T16<T>::vec4*)gu = pg;
+                    *(typename T16<T>::vec4*)(gu + 32) = pu;
+                }
             }
         } else {
 #pragma unroll
@@ -202,6 +210,14 @@ static void set_attrs() {
 #undef SETA
     mark_device_done(done_mask, cur_dev);
 }
+
+namespace vitg {
+int launch_gemm128_swiglu(GemmArgs g, int dtype, hipStream_t s) {
+    set_attrs();
+    g.tiles_m = ceil_div(g.M, BM); g.tiles_n = ceil_div(g.N, BN); g.group_m = 4; g.split_k = 1;
+    return dtype == DT_BF16 ? launch<bf16_t>(g, MODE_SWIGLU, s) : launch<f16_t>(g, MODE_SWIGLU, s);
+}
+}  // namespace vitg
 
 #if VITG_PROFILING_BUILD
 static unsigned long long* g_stamp_buf = nullptr;      // vitg_gemm_timeline_buffer

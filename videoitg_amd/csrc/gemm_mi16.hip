@@ -56,11 +56,16 @@ constexpr int MODE_RES16 = 3;      // internal: MODE_STORE16 with a residual pre
 // the same stage loop (the activation is recomputed); the main loop is the same code.  Separate instantiations: the default kernels do not carry it.
 // SAVE (vitg_swiglu with gu): the SwiGLU epilogue also writes the rounded accumulators - the pre-activations [32 gate | 32 up]... in the weight rows'
 // order - for the backward pass; silu(gate) * up itself still comes from the fp32 accumulators.
-template <typename T, int MODE, int BM, int BN, bool SK = false, int WM = 2, bool PATCH = false, bool SPLIT = false, bool SAVE = false>
+// WKM (vitg_swiglu_backward's dX = dGU W): the weight operand is K-major - W[k, n], k along the rows - so a K-tile of it is 64 rows of BN columns.  The LDS image
+// is those rows (BN * 2 bytes each, 32-B chunks XOR ((row >> 3) & 1) * 4 + (row & 3), again applied to the DMA's source address), and a fragment's 8
+// consecutive k of one column come from two ds_read_b64_tr_b16: a 16-lane group reads a 4 x 16 block (lane p: row p >> 2, columns 4 (p & 3) .. + 3) and
+// receives it transposed (lane p: column p, 4 rows).  The XOR puts the four rows of a group on four different 32-B bank ranges.
+template <typename T, int MODE, int BM, int BN, bool SK = false, int WM = 2, bool PATCH = false, bool SPLIT = false, bool SAVE = false, bool WKM = false>
 __global__ __launch_bounds__(G16_THREADS, 2) void gemm16_kernel(GemmArgs g_) {
     static_assert(!SK || MODE == MODE_F32, "stream-K partials are fp32 tiles");
     static_assert(!SPLIT || MODE == MODE_STORE16 || MODE == MODE_SWIGLU, "split pairs are a 16-bit-output form");
     static_assert(!PATCH || !SK, "the patch loader is not combined with stream-K");
+    static_assert(!WKM || (!SK && !PATCH && !SPLIT && !SAVE && MODE != MODE_SWIGLU), "the K-major weight operand is combined with the plain forms only");
     static_assert(!SAVE || (MODE == MODE_SWIGLU && !SPLIT), "pre-activations are saved by the plain SwiGLU form");
     typedef typename T16<T>::vec8 vec8;
     GemmArgs g = g_;
@@ -72,7 +77,7 @@ __global__ __launch_bounds__(G16_THREADS, 2) void gemm16_kernel(GemmArgs g_) {
             const int nk_all = g.K / 64, per = nk_all / g.split_k, rem = nk_all % g.split_k;
             const int k0 = sp * per + min(sp, rem);
             g.A = (const char*)g.A + (size_t)k0 * 128;
-            g.W = (const char*)g.W + (size_t)k0 * 128;
+            g.W = (const char*)g.W + (size_t)k0 * (WKM ? (size_t)g.ldw * 128 : (size_t)128);
             g.K = (per + (sp < rem ? 1 : 0)) * 64;
             g.out = (float*)g.out + (size_t)sp * g.split_stride;
         }
@@ -85,7 +90,7 @@ __global__ __launch_bounds__(G16_THREADS, 2) void gemm16_kernel(GemmArgs g_) {
     // 8 barriers per K-tile instead of 12): gate/up +4.2 % (1272 -> 1326 TF/s), step +0.3 %; the same on fc1 / o-proj: -1 % / +-0 (tools/archive/r03_calls.sh.txt (ab_mc6))
     // the 96-row wave tile (WM = 4 on 384 rows: MT = 6, NT = 8) runs intervals of 3 activation tiles x 8 weight tiles = 24 MFMAs, 8 barriers per K-tile
     // the 160-row wave tile (320 x 256, round 5: M = 1600 = 5 x 320 rows of one context-parallel rank): MT = 10 as two chunks of 5 = 20 MFMAs, 8 barriers per K-tile
-    constexpr int MC = MT == 10 ? 5 : MT == 6 ? 3 : (MODE == MODE_SWIGLU && MT == 12) ? 6 : 4;
+    constexpr int MC = WKM ? MT : MT == 10 ? 5 : MT == 6 ? 3 : (MODE == MODE_SWIGLU && MT == 12) ? 6 : 4;
     constexpr int NC = MT / MC;                          // row chunks per k-step
     constexpr int NI = 2 * NC;                           // intervals pairs per K-tile (2 k-steps of 32)
     constexpr int ROWB = 128;                            // bytes per LDS row: 64 k x 2 B
@@ -124,7 +129,8 @@ __global__ __launch_bounds__(G16_THREADS, 2) void gemm16_kernel(GemmArgs g_) {
     const int drow = lane >> 3, dslot = lane & 7;
     const int kfirst = SK ? (vb == 0 ? sk_k0 : 0) : 0;   // first K-tile of this work item
     const char* const a_base = (const char*)g.A + (size_t)m0 * g.lda * 2 + (size_t)kfirst * 128;
-    const char* const w_base = (const char*)g.W + (size_t)n0 * g.ldw * 2 + (size_t)kfirst * 128;
+    const char* const w_base = WKM ? (const char*)g.W + (size_t)n0 * 2 : (const char*)g.W + (size_t)n0 * g.ldw * 2 + (size_t)kfirst * 128;
+    const size_t w_step = WKM ? (size_t)g.ldw * 128 : (size_t)ROWB;      // bytes from one K-tile to the next
     unsigned a_cur[A_INSTR], w_cur[W_INSTR];
     int a_pair[PATCH ? A_INSTR : 1];                     // PATCH: which of the K-tile's four (c, ky) pairs this lane's chunk belongs to
 #pragma unroll
@@ -142,6 +148,12 @@ __global__ __launch_bounds__(G16_THREADS, 2) void gemm16_kernel(GemmArgs g_) {
     }
 #pragma unroll
     for (int j = 0; j < W_INSTR; ++j) {
+        if constexpr (WKM) {
+            const int idx = (wave * W_INSTR + j) * 64 + lane, row = idx / (BN / 8), slot = idx % (BN / 8);       // 16-B slots of a row
+            const int col = ((((slot >> 1) ^ (((row >> 3) & 1) * 4 + (row & 3))) << 1) + (slot & 1)) * 8;
+            w_cur[j] = ((unsigned)(row * g.ldw) + (unsigned)min(col, g.N - 8 - n0)) * 2u;     // (columns past N repeat the last ones: their outputs are not stored)
+            continue;
+        }
         const int R = (wave * W_INSTR + j) * 8 + drow;
         w_cur[j] = ((unsigned)(min(R, g.N - 1 - n0) * g.ldw) + (unsigned)((dslot ^ ((R >> 1) & 7)) << 3)) * 2u;
     }
@@ -149,7 +161,7 @@ __global__ __launch_bounds__(G16_THREADS, 2) void gemm16_kernel(GemmArgs g_) {
         char* st = smem + (kt & 1) * STAGE;
         const size_t koff = (size_t)kt * ROWB;
         const char* ka = a_base + koff;
-        const char* kw = w_base + koff;
+        const char* kw = w_base + (size_t)kt * w_step;
         unsigned off = j < A_INSTR ? a_cur[j] : w_cur[j - A_INSTR];
         if constexpr (PATCH) {
             if (j < A_INSTR) {                           // (pairs past 3 p - 1 are K padding: zero weight rows, any finite pixels)
@@ -181,8 +193,9 @@ __global__ __launch_bounds__(G16_THREADS, 2) void gemm16_kernel(GemmArgs g_) {
     // (the bias quads are requested here - older than every DMA in the vmcnt queue - and moved into the accumulators behind the wait for the first
     // stage, so the first DMA round trip covers them)
     f32x4 acc[NT][MT];
-    f32x4 bq[MODE == MODE_STORE16 ? NT : 1];
-    if constexpr (MODE == MODE_STORE16) {
+    constexpr bool BQ = MODE == MODE_STORE16 && !WKM;    // (the K-major form has no bias)
+    f32x4 bq[BQ ? NT : 1];
+    if constexpr (BQ) {
 #pragma unroll
         for (int i = 0; i < NT; ++i) {
             const int nb = n0 + wc * (NT * 16) + i * 16 + fq * 4;
@@ -252,6 +265,14 @@ __global__ __launch_bounds__(G16_THREADS, 2) void gemm16_kernel(GemmArgs g_) {
         }
     }
 
+    constexpr int RWB = BN * 2;                          // WKM: bytes per row of the weight tile
+    int t_off[WKM ? NT : 1];
+    if constexpr (WKM) {
+#pragma unroll
+        for (int i = 0; i < NT; ++i)
+            t_off[i] = A_BYTES + (fq * 8 + (r16 >> 2)) * RWB + (((wc * NT + i) ^ ((fq & 1) * 4 + (r16 >> 2))) << 5) + (r16 & 3) * 8;
+    }
+
     const int nk = SK ? (vb == 0 ? sk_c0 : sk_c1) : g.K / 64;
 #pragma unroll
     for (int j = 0; j < LPT; ++j) issue_one(0, j);
@@ -259,7 +280,7 @@ __global__ __launch_bounds__(G16_THREADS, 2) void gemm16_kernel(GemmArgs g_) {
     vec8 fw[NT], fa[MC];
     const bool grpB = wave >= 4;
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    if constexpr (MODE == MODE_STORE16) {
+    if constexpr (BQ) {
 #pragma unroll
         for (int i = 0; i < NT; ++i)
 #pragma unroll
@@ -282,7 +303,14 @@ __global__ __launch_bounds__(G16_THREADS, 2) void gemm16_kernel(GemmArgs g_) {
             const int ks = ph / NC, c = ph % NC;
             if (c == 0) {
 #pragma unroll
-                for (int i = 0; i < NT; ++i) fw[i] = *(const vec8*)(st_ + w_off[ks] + i * (16 * ROWB));
+                for (int i = 0; i < NT; ++i) {
+                    if constexpr (WKM) {
+                        typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+                        const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(st_ + t_off[i] + ks * (32 * RWB)));
+                        const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(st_ + t_off[i] + ks * (32 * RWB) + 4 * RWB));
+                        fw[i] = bitcast<vec8>(__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+                    } else fw[i] = *(const vec8*)(st_ + w_off[ks] + i * (16 * ROWB));
+                }
             }
 #pragma unroll
             for (int i = 0; i < MC; ++i) fa[i] = *(const vec8*)(st_ + a_off[ks] + (c * MC + i) * (16 * ROWB));
@@ -549,14 +577,14 @@ __global__ __launch_bounds__(G16_THREADS, 2) void gemm16_kernel(GemmArgs g_) {
     }   // tile loop
 }
 
-template <typename T, int MODE, int BM, int BN, int WM = 2, bool SPLIT = false, bool SAVE = false>
+template <typename T, int MODE, int BM, int BN, int WM = 2, bool SPLIT = false, bool SAVE = false, bool WKM = false>
 static int launch16(GemmArgs g, hipStream_t s) {
     constexpr int lds = 2 * (BM + BN) * 128;
     static int done_dev[16] = {0};                       // per device: the attribute belongs to the device's copy of the kernel
     int cur_dev = 0;
     (void)hipGetDevice(&cur_dev);
     if (cur_dev >= 16 || !done_dev[cur_dev]) {
-        (void)hipFuncSetAttribute((const void*)gemm16_kernel<T, MODE, BM, BN, false, WM, false, SPLIT, SAVE>, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+        (void)hipFuncSetAttribute((const void*)gemm16_kernel<T, MODE, BM, BN, false, WM, false, SPLIT, SAVE, WKM>, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
         if (cur_dev < 16) done_dev[cur_dev] = 1;
     }
     g.tiles_m = ceil_div(g.M, BM);
@@ -572,7 +600,7 @@ static int launch16(GemmArgs g, hipStream_t s) {
     // one block per CU walking the tile list when there are at least two tiles per CU (gemm256.hip: "software relaunch")
     const bool loop = nwg >= 2 * cus && !(RESEARCH(gemm_flags) & 0x1000000);
     const int splits = (MODE == MODE_F32 && g.split_k > 1) ? g.split_k : 1;
-    hipLaunchKernelGGL((gemm16_kernel<T, MODE, BM, BN, false, WM, false, SPLIT, SAVE>), dim3(loop && splits == 1 ? cus : nwg, splits), dim3(G16_THREADS), lds, s, g);
+    hipLaunchKernelGGL((gemm16_kernel<T, MODE, BM, BN, false, WM, false, SPLIT, SAVE, WKM>), dim3(loop && splits == 1 ? cus : nwg, splits), dim3(G16_THREADS), lds, s, g);
     return (int)hipGetLastError();
 }
 
@@ -590,6 +618,16 @@ int launch_gemm_mi16_swiglu_save(const GemmArgs& g, int dtype, hipStream_t s) {
         if (cfg == 10 && g.M >= 384) return launch16<T, MODE_SWIGLU, 384, 256, 2, false, true>(g, s);
         if (cfg == 12 && g.M > 256) return launch16<T, MODE_SWIGLU, 320, 256, 2, false, true>(g, s);
         return launch16<T, MODE_SWIGLU, 256, 256, 2, false, true>(g, s);
+    };
+    return dtype == DT_BF16 ? run(bf16_t{}) : run(f16_t{});
+}
+
+// C = A[M,K] . W[K,N]: the weight operand K-major.  g.split_k > 1: raw fp32 partials of the K ranges into g.out (split_stride apart); else 16-bit output
+int launch_gemm_mi16_kmajor(const GemmArgs& g, int dtype, int bm, hipStream_t s) {
+    auto run = [&](auto t) {
+        typedef decltype(t) T;
+        if (g.split_k > 1) return bm == 320 ? launch16<T, MODE_F32, 320, 256, 2, false, false, true>(g, s) : launch16<T, MODE_F32, 256, 256, 2, false, false, true>(g, s);
+        return launch16<T, MODE_STORE16, 256, 256, 2, false, false, true>(g, s);
     };
     return dtype == DT_BF16 ? run(bf16_t{}) : run(f16_t{});
 }

@@ -9,6 +9,7 @@
 // there, so neither large nor tiny gradients change the norm, and the fixed order gives the same bits on every call.
 #include "train_common.h"
 #include <math.h>
+#include <stdlib.h>
 
 namespace vitg {
 
@@ -39,12 +40,24 @@ __device__ __forceinline__ double clip_sum_piece(const T* __restrict__ p, long c
     long done = 0;
     if (((uintptr_t)p & 15) == 0) {
         done = count / V * V;
-        for (long i = (long)tid * V; i < done; i += CLIP_THREADS * V) {
+        long i = (long)tid * V;
+        double q[4] = {0.0, 0.0, 0.0, 0.0};
+        for (; i + 3 * CLIP_THREADS * V < done; i += 4 * CLIP_THREADS * V) {       // four loads in flight, four chains of sums
+            float v[4][V];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) load_vec<T, V>(p + i + u * CLIP_THREADS * V, v[u]);
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+#pragma unroll
+                for (int e = 0; e < V; ++e) q[u] += (double)v[u][e] * (double)v[u][e];
+        }
+        for (; i < done; i += CLIP_THREADS * V) {
             float v[V];
             load_vec<T, V>(p + i, v);
 #pragma unroll
-            for (int e = 0; e < V; ++e) s += (double)v[e] * (double)v[e];
+            for (int e = 0; e < V; ++e) q[0] += (double)v[e] * (double)v[e];
         }
+        s = (q[0] + q[1]) + (q[2] + q[3]);
     }
     for (long i = done + tid; i < count; i += CLIP_THREADS) { const double v = (double)(float)p[i]; s += v * v; }
     return s;
@@ -77,12 +90,24 @@ __global__ __launch_bounds__(CLIP_THREADS) void grad_sumsq_kernel(const ClipArgs
 }
 
 template <typename T>
-__device__ __forceinline__ void clip_scale_piece(const T* __restrict__ p, T* __restrict__ q, long count, float factor, int tid) {
+__device__ __forceinline__ void clip_scale_piece(const T* p, T* q, long count, float factor, int tid) {
     constexpr int V = 16 / sizeof(T);
     long done = 0;
     if ((((uintptr_t)p | (uintptr_t)q) & 15) == 0) {
         done = count / V * V;
-        for (long i = (long)tid * V; i < done; i += CLIP_THREADS * V) {
+        long i = (long)tid * V;
+        for (; i + 3 * CLIP_THREADS * V < done; i += 4 * CLIP_THREADS * V) {
+            float v[4][V];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) load_vec<T, V>(p + i + u * CLIP_THREADS * V, v[u]);
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+#pragma unroll
+                for (int e = 0; e < V; ++e) v[u][e] *= factor;
+                store_vec<T, V>(q + i + u * CLIP_THREADS * V, v[u]);
+            }
+        }
+        for (; i < done; i += CLIP_THREADS * V) {
             float v[V];
             load_vec<T, V>(p + i, v);
 #pragma unroll
@@ -161,6 +186,39 @@ static int clip_fill(ClipArgs& a, int first, int count, const void* const* in, v
     return end;
 }
 
+struct ClipSpan { uintptr_t begin, end; bool written; };
+static int clip_span_order(const void* a, const void* b) {
+    const uintptr_t x = ((const ClipSpan*)a)->begin, y = ((const ClipSpan*)b)->begin;
+    return x < y ? -1 : x > y ? 1 : 0;
+}
+// whether memory that the call writes - outputs, norm, workspace - is also another tensor's (a shared byte would be scaled twice, or before another block has
+// read it).  In order of their begins, a span that meets any earlier one meets the one that reaches furthest; if the pair in question is another one, that
+// one and its partner have met before.
+static bool clip_overlaps(int count, const void* const* in, void* const* out, const long* numel, const int* dtype, const void* norm, const void* ws, long ws_bytes,
+                          bool* failed) {
+    ClipSpan* const sp = (ClipSpan*)malloc(sizeof(ClipSpan) * (2 * (size_t)count + 2));
+    *failed = sp == nullptr;
+    if (!sp) return false;
+    int n = 0;
+    for (int i = 0; i < count; ++i) {
+        const size_t bytes = (size_t)numel[i] * dtype_size(dtype[i]);
+        if (!bytes) continue;
+        sp[n++] = {(uintptr_t)in[i], (uintptr_t)in[i] + bytes, out && out[i] == in[i]};
+        if (out && out[i] != in[i]) sp[n++] = {(uintptr_t)out[i], (uintptr_t)out[i] + bytes, true};
+    }
+    sp[n++] = {(uintptr_t)norm, (uintptr_t)norm + 4, true};
+    sp[n++] = {(uintptr_t)ws, (uintptr_t)ws + (size_t)ws_bytes, true};
+    qsort(sp, n, sizeof(ClipSpan), clip_span_order);
+    bool meet = false;
+    int far = 0;
+    for (int i = 1; i < n && !meet; ++i) {
+        meet = sp[i].begin < sp[far].end && (sp[i].written || sp[far].written);
+        if (sp[i].end > sp[far].end) far = i;
+    }
+    free(sp);
+    return meet;
+}
+
 static int clip_check(int count, const void* const* in, void* const* out, const long* numel, const int* dtype) {
     if (count < 0) return VITG_ERR_SHAPE;
     if (count && (!in || !numel || !dtype)) return VITG_ERR_ARG;
@@ -202,6 +260,8 @@ extern "C" int vitg_clip_grad(int count, const void* const* grads, void* const* 
     long need = 0;
     (void)vitg_clip_grad_plan(count, numel, dtype, &need);
     if (workspace_bytes < need) return VITG_ERR_ARG;
+    bool failed = false;
+    if (clip_overlaps(count, grads, outs, numel, dtype, norm, workspace, need, &failed) || failed) return VITG_ERR_ARG;
     hipStream_t s = (hipStream_t)stream;
     double* const sums = (double*)workspace;
     ClipArgs a;

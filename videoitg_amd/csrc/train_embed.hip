@@ -33,15 +33,69 @@ __global__ void embed_lookup_kernel(const long long* __restrict__ ids, long n, c
 }
 
 // ---- stable sort of (key, position); key = id, or vocab for a slot without a token (sorts behind every id) ------------------------
+// The dense form also has to zero every row of the table (the rows of the batch's tokens are overwritten by the sums): a write of the whole table, which
+// keeps HBM busy while the sort uses a few CUs.  So the zeroing rides along: each sort launch carries extra blocks behind its own that zero a share of the rows.
+struct ZeroRows { void* table; long pitch, bytes, begin, end; int blocks; };      // rows [begin, end), `bytes` of every `pitch`, by the last `blocks` of the grid
+__device__ __forceinline__ void zero_rows(const ZeroRows& z, int block) {
+    if ((z.pitch | z.bytes | (long)(uintptr_t)z.table) & 15) {
+        for (long r = z.begin + block; r < z.end; r += z.blocks)
+            for (long c = threadIdx.x * 8l; c < z.bytes; c += blockDim.x * 8l) *(u32x2*)((char*)z.table + r * z.pitch + c) = u32x2{0, 0};
+    } else {
+        for (long r = z.begin + block; r < z.end; r += z.blocks)
+            for (long c = threadIdx.x * 16l; c < z.bytes; c += blockDim.x * 16l) *(u32x4*)((char*)z.table + r * z.pitch + c) = u32x4{0, 0, 0, 0};
+    }
+}
+__global__ __launch_bounds__(256) void zero_rows_kernel(const ZeroRows z) { zero_rows(z, blockIdx.x); }
+
 constexpr int SORT_BITS = 9, SORT_BINS = 1 << SORT_BITS, SORT_TILE = 2048, SORT_THREADS = 256;
 
 __device__ __forceinline__ unsigned sort_key(long long id, unsigned vocab) { return id >= 0 && id < (long long)vocab ? (unsigned)id : vocab; }
 
-// one least-significant-digit pass = two launches: digit counts per tile of 2048 keys, then every tile scatters its keys behind the counts of the smaller
+// Short lists (n <= RANK_MAX): a token's place is the number of smaller keys plus the number of equal keys in front of it, counted against all keys in LDS.
+// 64 tokens per block, its 16 waves count a sixteenth of the list each.  n^2 / 2 comparisons, two instructions each, on all CUs - and one launch.
+constexpr int RANK_MAX = 15360, RANK_WAVES = 16;         // 60 KiB of keys
+__global__ __launch_bounds__(RANK_WAVES * 64) void sort_rank_kernel(const long long* __restrict__ ids, int n, unsigned vocab, unsigned* __restrict__ key_out,
+                                                                    unsigned* __restrict__ pos_out, int blocks, const ZeroRows z) {
+    extern __shared__ __attribute__((aligned(16))) unsigned keys[];      // n keys, padded to a multiple of 16 with the largest value
+    if ((int)blockIdx.x >= blocks) { zero_rows(z, (int)blockIdx.x - blocks); return; }
+    __shared__ unsigned part[64];
+    const int padded = (n + 15) & ~15;
+#pragma unroll 4
+    for (int i = threadIdx.x; i < padded; i += RANK_WAVES * 64) keys[i] = i < n ? sort_key(ids[i], vocab) : 0xffffffffu;
+    if (threadIdx.x < 64) part[threadIdx.x] = 0;
+    __syncthreads();
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int i0 = blockIdx.x * 64, i = i0 + lane;
+    const unsigned mine = keys[min(i, n - 1)];
+    const int per = (padded / 16 + RANK_WAVES - 1) / RANK_WAVES * 16, lo = min(wave * per, padded), hi = min(lo + per, padded);
+    unsigned count = 0;
+    auto span = [&](int a, int b, auto f) {              // [a, b) of this wave's share; all bounds are multiples of 16
+        for (int j = max(a, lo); j < min(b, hi); j += 16) {
+            u32x4 k[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) k[u] = *(const u32x4*)(keys + j + u * 4);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) count += f(k[e >> 2][e & 3], j + e) ? 1u : 0u;
+        }
+    };
+    span(0, i0, [&](unsigned k, int) { return k <= mine; });
+    span(i0, min(i0 + 64, padded), [&](unsigned k, int j) { return k < mine || (k == mine && j < i); });
+    span(i0 + 64, padded, [&](unsigned k, int) { return k < mine; });
+    atomicAdd(&part[lane], count);                       // whole numbers: the order does not matter
+    __syncthreads();
+    if (wave == 0 && i < n) {
+        const unsigned at = part[lane];
+        key_out[at] = mine;
+        pos_out[at] = (unsigned)i;
+    }
+}
+
+// Longer lists: radix passes, least significant digit first.  One pass = two launches: digit counts per tile of 2048 keys, then every tile scatters its keys behind the counts of the smaller
 // digits and of the tiles in front of it.  FIRST: the keys are the ids themselves, the positions 0 .. n-1.
 template <bool FIRST>
 __global__ __launch_bounds__(SORT_THREADS) void sort_count_kernel(const long long* __restrict__ ids, const unsigned* __restrict__ key_in, long n, unsigned vocab,
-                                                                  int shift, unsigned* __restrict__ counts) {
+                                                                  int shift, unsigned* __restrict__ counts, int tiles, const ZeroRows z) {
+    if ((int)blockIdx.x >= tiles) { zero_rows(z, (int)blockIdx.x - tiles); return; }
     __shared__ unsigned bins[SORT_BINS];
     for (int b = threadIdx.x; b < SORT_BINS; b += SORT_THREADS) bins[b] = 0;
     __syncthreads();
@@ -57,7 +111,9 @@ __global__ __launch_bounds__(SORT_THREADS) void sort_count_kernel(const long lon
 template <bool FIRST>
 __global__ __launch_bounds__(SORT_THREADS) void sort_scatter_kernel(const long long* __restrict__ ids, const unsigned* __restrict__ key_in,
                                                                     const unsigned* __restrict__ pos_in, long n, unsigned vocab, int shift, int tiles,
-                                                                    const unsigned* __restrict__ counts, unsigned* __restrict__ key_out, unsigned* __restrict__ pos_out) {
+                                                                    const unsigned* __restrict__ counts, unsigned* __restrict__ key_out, unsigned* __restrict__ pos_out,
+                                                                    const ZeroRows z) {
+    if ((int)blockIdx.x >= tiles) { zero_rows(z, (int)blockIdx.x - tiles); return; }
     constexpr int WAVES = SORT_THREADS / 64, ROUNDS = SORT_TILE / SORT_THREADS, BPT = SORT_BINS / SORT_THREADS;
     __shared__ unsigned next[WAVES][SORT_BINS];          // next free slot of a digit for one wave's keys
     __shared__ unsigned wave_total[WAVES];
@@ -128,16 +184,6 @@ __global__ __launch_bounds__(SORT_THREADS) void sort_scatter_kernel(const long l
 }
 
 // ---- the sums ----------------------------------------------------------------------------------------------------------------------
-// zero rows of the dense form (accumulate = 0): the rows of the batch's tokens are overwritten by the kernels below
-template <int V, typename T>
-__global__ __launch_bounds__(256) void zero_rows_kernel(T* __restrict__ table, long ldt, long rows, int cv) {
-    float z[V];
-#pragma unroll
-    for (int e = 0; e < V; ++e) z[e] = 0.f;
-    for (long r = blockIdx.x; r < rows; r += gridDim.x)
-        for (int c = threadIdx.x; c < cv; c += 256) store_vec<T, V>(table + r * ldt + (long)c * V, z);
-}
-
 template <typename TT, int V>
 __device__ __forceinline__ void finish_row(TT* __restrict__ row, int accumulate, float scale, const float (&acc)[V]) {
     float v[V];
@@ -161,40 +207,61 @@ __global__ __launch_bounds__(256) void embed_grad_kernel(const unsigned* __restr
     float acc[V];
 #pragma unroll
     for (int e = 0; e < V; ++e) acc[e] = 0.f;
-    for (long e = e0; e < e1; ++e) {
-        float v[V];
-        load_vec<TD, V>(dout + (long)pos[e] * ldd + (long)c * V, v);
+    constexpr int G = 4;                                 // rows in flight
+    for (long e4 = e0; e4 < e1; e4 += G) {
+        float v[G][V];
+        unsigned after[G];
 #pragma unroll
-        for (int k = 0; k < V; ++k) acc[k] += v[k];
-        const unsigned after = e + 1 < n ? key[e + 1] : vocab;
-        if (after != run) {                              // the run ends with this token
-            if (began) finish_row<TT, V>(table + (long)run * ldt + (long)c * V, accumulate, scale, acc);
-            else store_vec<float, V>(partial + ((size_t)blockIdx.x * 2) * ((size_t)cv * V) + (size_t)c * V, acc);
-            if (after >= vocab) return;
-            run = after;
-            began = true;
+        for (int g = 0; g < G; ++g) {
+            const long e = min(e4 + g, e1 - 1);
+            load_vec<TD, V>(dout + (long)pos[e] * ldd + (long)c * V, v[g]);
+            after[g] = e + 1 < n ? key[e + 1] : vocab;
+        }
 #pragma unroll
-            for (int k = 0; k < V; ++k) acc[k] = 0.f;
-            if (e + 1 == e1) return;                     // the next run starts the next chunk
+        for (int g = 0; g < G; ++g) {
+            if (e4 + g >= e1) break;
+#pragma unroll
+            for (int k = 0; k < V; ++k) acc[k] += v[g][k];
+            if (after[g] != run) {                       // the run ends with this token
+                if (began) finish_row<TT, V>(table + (long)run * ldt + (long)c * V, accumulate, scale, acc);
+                else store_vec<float, V>(partial + ((size_t)blockIdx.x * 2) * ((size_t)cv * V) + (size_t)c * V, acc);
+                if (after[g] >= vocab || e4 + g + 1 == e1) return;      // no token is left, or the next run starts the next chunk
+                run = after[g];
+                began = true;
+#pragma unroll
+                for (int k = 0; k < V; ++k) acc[k] = 0.f;
+            }
         }
     }
     // the run goes on in the next chunk
     store_vec<float, V>(partial + ((size_t)blockIdx.x * 2 + (began ? 1 : 0)) * ((size_t)cv * V) + (size_t)c * V, acc);
 }
 
-// runs across chunks: the block of the chunk in which a run begins adds its partials in chunk order - the waves take consecutive parts of the list,
-// their sums join through LDS in wave order
-constexpr int JOIN_WAVES = 8;
+// runs across chunks: the block of the chunk in which a run begins adds its partials in chunk order.  16 waves: four column groups of 256 columns, four
+// consecutive parts of the list each; the parts' sums join through LDS in order
+constexpr int JOIN_PARTS = 4, JOIN_COLS = 1024;
 template <typename TT>
-__global__ __launch_bounds__(JOIN_WAVES * 64) void embed_join_kernel(const unsigned* __restrict__ key, long n, unsigned vocab, int chunk, int D, float scale,
-                                                                     TT* __restrict__ table, long ldt, int accumulate, const float* __restrict__ partial) {
+__global__ __launch_bounds__(1024) void embed_join_kernel(const unsigned* __restrict__ key, long n, unsigned vocab, int chunk, int D, float scale,
+                                                          TT* __restrict__ table, long ldt, int accumulate, const float* __restrict__ partial) {
     constexpr int V = 4;
-    __shared__ float part[JOIN_WAVES][64 * V];
-    const long b = blockIdx.x, chunks = (n + chunk - 1) / chunk;
-    if (b + 1 >= chunks) return;
+    __shared__ float part[JOIN_PARTS][JOIN_COLS];
+    __shared__ unsigned begins[16];
+    const long chunks = (n + chunk - 1) / chunk;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, p = wave >> 2;
+    if (lane == 0) {                                     // wave w looks at chunk 16 blockIdx.x + w: does a run that goes on behind it begin there
+        const long b = blockIdx.x * 16l + wave;
+        unsigned is = 0;
+        if (b + 1 < chunks) {
+            const unsigned run = key[(b + 1) * chunk - 1];
+            is = run < vocab && key[(b + 1) * chunk] == run && !(b > 0 && key[b * chunk - 1] == run);
+        }
+        begins[wave] = is;
+    }
+    __syncthreads();
+    for (int w16 = 0; w16 < 16; ++w16) {
+    if (!begins[w16]) continue;                          // (the same for every thread of the block)
+    const long b = blockIdx.x * 16l + w16;
     const unsigned run = key[(b + 1) * chunk - 1];
-    if (run >= vocab || key[(b + 1) * chunk] != run || (b > 0 && key[b * chunk - 1] == run)) return;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     long last = b + 1;                                   // last chunk that holds a part of the run
     for (;;) {
         const long j = last + 1 + lane;
@@ -203,23 +270,38 @@ __global__ __launch_bounds__(JOIN_WAVES * 64) void embed_join_kernel(const unsig
         last += more;
         if (more < 64) break;
     }
-    const int c = (blockIdx.y * 64 + lane) * V;
-    const long items = last - b + 1, per = (items + JOIN_WAVES - 1) / JOIN_WAVES;
+    const int at = (wave & 3) * 256 + lane * V, c = blockIdx.y * JOIN_COLS + at;
+    const long items = last - b + 1, per = (items + JOIN_PARTS - 1) / JOIN_PARTS, i0 = p * per, i1 = min(i0 + per, items);
     float acc[V] = {0.f, 0.f, 0.f, 0.f};
-    if (c < D)
-        for (long i = wave * per; i < min((wave + 1) * per, items); ++i) {
+    if (c < D) {
+        // item i: the part that chunk b + i holds (slot 1 of the first, slot 0 of the others)
+        auto item = [&](long i) { return partial + ((size_t)(b + i) * 2 + (i == 0 ? 1 : 0)) * (size_t)D + c; };
+        long i = i0;
+        for (; i + 8 <= i1; i += 8) {
+            float v[8][V];
+#pragma unroll
+            for (int g = 0; g < 8; ++g) load_vec<float, V>(item(i + g), v[g]);
+#pragma unroll
+            for (int g = 0; g < 8; ++g)
+#pragma unroll
+                for (int k = 0; k < V; ++k) acc[k] += v[g][k];
+        }
+        for (; i < i1; ++i) {
             float v[V];
-            load_vec<float, V>(partial + ((size_t)(b + i) * 2 + (i == 0 ? 1 : 0)) * (size_t)D + c, v);
+            load_vec<float, V>(item(i), v);
 #pragma unroll
             for (int k = 0; k < V; ++k) acc[k] += v[k];
         }
-    store_vec<float, V>(&part[wave][lane * V], acc);
+    }
+    store_vec<float, V>(&part[p][at], acc);
     __syncthreads();
-    if (wave == 0 && c < D) {
-        for (int w = 1; w < JOIN_WAVES; ++w)
+    if (p == 0 && c < D) {
+        for (int w = 1; w < JOIN_PARTS; ++w)
 #pragma unroll
-            for (int k = 0; k < V; ++k) acc[k] += part[w][lane * V + k];
+            for (int k = 0; k < V; ++k) acc[k] += part[w][at + k];
         finish_row<TT, V>(table + (long)run * ldt + c, accumulate, scale, acc);
+    }
+    __syncthreads();
     }
 }
 
@@ -229,13 +311,13 @@ static size_t round256(size_t b) { return (b + 255) & ~(size_t)255; }
 
 struct EmbedWorkspace { size_t key[2], pos[2], counts, partial, bytes; int tiles, chunk; long chunks; };
 static EmbedWorkspace embed_workspace(long n, int D) {
-    EmbedWorkspace w;
+    EmbedWorkspace w = {};
     w.tiles = (int)((n + SORT_TILE - 1) / SORT_TILE);
     w.chunk = embed_chunk(n);
     w.chunks = (n + w.chunk - 1) / w.chunk;
     size_t at = 0;
     for (int i = 0; i < 2; ++i) { w.key[i] = at; at += round256((size_t)n * 4); w.pos[i] = at; at += round256((size_t)n * 4); }
-    w.counts = at; at += round256((size_t)w.tiles * SORT_BINS * 4);
+    if (n > RANK_MAX) { w.counts = at; at += round256((size_t)w.tiles * SORT_BINS * 4); }
     w.partial = at; at += round256((size_t)w.chunks * 2 * D * 4);
     w.bytes = at;
     return w;
@@ -284,16 +366,12 @@ extern "C" int vitg_embed_backward(const long long* ids, long n, const void* dou
     const EmbedWorkspace w = n ? embed_workspace(n, D) : EmbedWorkspace{};
     if (n && (workspace_bytes < (long)w.bytes || !aligned_to(workspace, 16))) return VITG_ERR_ARG;
     hipStream_t s = (hipStream_t)stream;
-    if (!accumulate) {
-        const bool wide = D % 8 == 0 && ldt % 8 == 0 && aligned_to(dtable, 16);
-        const unsigned grid = (unsigned)(vocab < 8192 ? vocab : 8192);
-        with_dtype(table_dtype, [&](auto tt) {
-            typedef decltype(tt) TT;
-            if (wide) hipLaunchKernelGGL((zero_rows_kernel<8, TT>), dim3(grid), dim3(256), 0, s, (TT*)dtable, ldt, vocab, D / 8);
-            else hipLaunchKernelGGL((zero_rows_kernel<4, TT>), dim3(grid), dim3(256), 0, s, (TT*)dtable, ldt, vocab, D / 4);
-        });
+    const int tsize = dtype_size(table_dtype);
+    if (n == 0) {
+        const ZeroRows z = {dtable, ldt * tsize, (long)D * tsize, 0, vocab, 2048};
+        if (!accumulate) hipLaunchKernelGGL(zero_rows_kernel, dim3(2048), dim3(256), 0, s, z);
+        return launched();
     }
-    if (n == 0) return launched();
     char* const base = (char*)workspace;
     unsigned *key[2], *pos[2], *counts = (unsigned*)(base + w.counts);
     for (int i = 0; i < 2; ++i) { key[i] = (unsigned*)(base + w.key[i]); pos[i] = (unsigned*)(base + w.pos[i]); }
@@ -301,18 +379,32 @@ extern "C" int vitg_embed_backward(const long long* ids, long n, const void* dou
     int bits = 1;
     while ((vocab >> bits) != 0) ++bits;                 // keys 0 .. vocab
     const unsigned v = (unsigned)vocab;
+    // launch i of the sort zeroes rows [i vocab / launches, (i + 1) vocab / launches)
+    const int passes = (bits + SORT_BITS - 1) / SORT_BITS, launches = n <= RANK_MAX ? 1 : 2 * passes;
+    auto zero = [&](int i) {
+        ZeroRows z = {dtable, ldt * tsize, (long)D * tsize, vocab * i / launches, vocab * (i + 1) / launches, 0};
+        if (!accumulate) z.blocks = (int)(z.end - z.begin < 2048 ? z.end - z.begin : 2048);
+        return z;
+    };
     int cur = 0;
-    for (int shift = 0, pass = 0; shift < bits; shift += SORT_BITS, ++pass) {
-        const int to = cur ^ 1;
-        if (pass == 0) {
-            hipLaunchKernelGGL(sort_count_kernel<true>, dim3(w.tiles), dim3(SORT_THREADS), 0, s, ids, nullptr, n, v, shift, counts);
-            hipLaunchKernelGGL(sort_scatter_kernel<true>, dim3(w.tiles), dim3(SORT_THREADS), 0, s, ids, nullptr, nullptr, n, v, shift, w.tiles, counts, key[to], pos[to]);
-        } else {
-            hipLaunchKernelGGL(sort_count_kernel<false>, dim3(w.tiles), dim3(SORT_THREADS), 0, s, nullptr, key[cur], n, v, shift, counts);
-            hipLaunchKernelGGL(sort_scatter_kernel<false>, dim3(w.tiles), dim3(SORT_THREADS), 0, s, nullptr, key[cur], pos[cur], n, v, shift, w.tiles, counts, key[to], pos[to]);
+    if (launches == 1) {
+        const int blocks = (int)((n + 63) / 64);
+        const ZeroRows z = zero(0);
+        hipLaunchKernelGGL(sort_rank_kernel, dim3(blocks + z.blocks), dim3(RANK_WAVES * 64), (size_t)((n + 15) & ~15l) * 4, s, ids, (int)n, v, key[0], pos[0], blocks, z);
+    } else
+        for (int p = 0; p < passes; ++p) {
+            const int to = cur ^ 1, shift = p * SORT_BITS;
+            const ZeroRows z0 = zero(2 * p), z1 = zero(2 * p + 1);
+            const dim3 g0(w.tiles + z0.blocks), g1(w.tiles + z1.blocks), t(SORT_THREADS);
+            if (p == 0) {
+                hipLaunchKernelGGL(sort_count_kernel<true>, g0, t, 0, s, ids, nullptr, n, v, shift, counts, w.tiles, z0);
+                hipLaunchKernelGGL(sort_scatter_kernel<true>, g1, t, 0, s, ids, nullptr, nullptr, n, v, shift, w.tiles, counts, key[to], pos[to], z1);
+            } else {
+                hipLaunchKernelGGL(sort_count_kernel<false>, g0, t, 0, s, nullptr, key[cur], n, v, shift, counts, w.tiles, z0);
+                hipLaunchKernelGGL(sort_scatter_kernel<false>, g1, t, 0, s, nullptr, key[cur], pos[cur], n, v, shift, w.tiles, counts, key[to], pos[to], z1);
+            }
+            cur = to;
         }
-        cur = to;
-    }
     const bool wide = D % 8 == 0 && ldt % 8 == 0 && ldd % 8 == 0 && aligned_to(dtable, 16) && aligned_to(dout, 16);
     const int cv = D / (wide ? 8 : 4);
     with_dtype(dout_dtype, [&](auto td) {
@@ -327,7 +419,7 @@ extern "C" int vitg_embed_backward(const long long* ids, long n, const void* dou
     if (w.chunks > 1)
         with_dtype(table_dtype, [&](auto tt) {
             typedef decltype(tt) TT;
-            hipLaunchKernelGGL((embed_join_kernel<TT>), dim3((unsigned)w.chunks, ceil_div(D, 256)), dim3(JOIN_WAVES * 64), 0, s, key[cur], n, v, w.chunk, D, scale, (TT*)dtable, ldt, accumulate, partial);
+            hipLaunchKernelGGL((embed_join_kernel<TT>), dim3((unsigned)((w.chunks + 15) / 16), ceil_div(D, JOIN_COLS)), dim3(1024), 0, s, key[cur], n, v, w.chunk, D, scale, (TT*)dtable, ldt, accumulate, partial);
         });
     return launched();
 }

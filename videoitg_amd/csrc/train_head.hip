@@ -11,14 +11,15 @@
 
 namespace vitg {
 
-template <typename T, int V>
+// One block per frame when there are enough frames to fill the chip; otherwise the columns of a frame are spread over gridDim.y blocks (SCORE = false) and
+// pool_dot_kernel takes the scores from the means.
+template <typename T, int V, bool SCORE>
 __global__ __launch_bounds__(1024) void pool_score_save_kernel(const T* __restrict__ h, long ldh, int tokens, int cv, const float* __restrict__ w,
                                                                const float* __restrict__ b, float* __restrict__ logits, float* __restrict__ pooled, long ldp) {
-    __shared__ float part[16];
     const long t = blockIdx.x;
     const float inv = 1.0f / (float)tokens;
     float dot = 0.f;
-    for (int c = threadIdx.x; c < cv; c += blockDim.x) {
+    for (int c = blockIdx.y * blockDim.x + threadIdx.x; c < cv; c += gridDim.y * blockDim.x) {
         const T* const p = h + t * tokens * ldh + (long)c * V;
         float s[V];
 #pragma unroll
@@ -30,20 +31,45 @@ __global__ __launch_bounds__(1024) void pool_score_save_kernel(const T* __restri
 #pragma unroll
             for (int e = 0; e < V; ++e) s[e] += v[e];
         }
-        float ww[V];
-        load_vec<float, V>(w + c * V, ww);
 #pragma unroll
-        for (int e = 0; e < V; ++e) { s[e] *= inv; dot += s[e] * ww[e]; }
+        for (int e = 0; e < V; ++e) s[e] *= inv;
         store_vec<float, V>(pooled + t * ldp + (long)c * V, s);
+        if constexpr (SCORE) {
+            float ww[V];
+            load_vec<float, V>(w + c * V, ww);
+#pragma unroll
+            for (int e = 0; e < V; ++e) dot += s[e] * ww[e];
+        }
+    }
+    if constexpr (SCORE) {
+        __shared__ float part[16];
+        dot = wave_sum(dot);
+        if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = dot;
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            float sum = 0.f;
+            for (int i = 0; i < (int)(blockDim.x >> 6); ++i) sum += part[i];
+            logits[t] = sum + b[0];
+        }
+    }
+}
+
+__global__ __launch_bounds__(256) void pool_dot_kernel(const float* __restrict__ pooled, long ldp, int D, const float* __restrict__ w, const float* __restrict__ b,
+                                                       float* __restrict__ logits) {
+    __shared__ float part[4];
+    const float* const p = pooled + (long)blockIdx.x * ldp;
+    float dot = 0.f;
+    for (int c = threadIdx.x * 4; c < D; c += 1024) {
+        float v[4], ww[4];
+        load_vec<float, 4>(p + c, v);
+        load_vec<float, 4>(w + c, ww);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) dot += v[e] * ww[e];
     }
     dot = wave_sum(dot);
     if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = dot;
     __syncthreads();
-    if (threadIdx.x == 0) {
-        float sum = 0.f;
-        for (int i = 0; i < (int)(blockDim.x >> 6); ++i) sum += part[i];
-        logits[t] = sum + b[0];
-    }
+    if (threadIdx.x == 0) logits[blockIdx.x] = part[0] + part[1] + part[2] + part[3] + b[0];
 }
 
 __device__ __forceinline__ double block_sum_1024(double v, double* red) {
@@ -147,12 +173,19 @@ extern "C" int vitg_pool_score_save(const void* h, int h_dtype, long ldh, int fr
     if (tokens_per_frame <= 0 || D <= 0 || ldh < D || ldp < D) return VITG_ERR_SHAPE;
     if (D % 4 || ldh % 4 || ldp % 4 || !aligned_to(h, 4 * dtype_size(h_dtype)) || !aligned_to(w, 16) || !aligned_to(pooled, 16)) return VITG_ERR_ALIGN;
     const bool wide = h_dtype != DT_F32 && D % 8 == 0 && ldh % 8 == 0 && aligned_to(h, 16);
-    const int cv = D / (wide ? 8 : 4), threads = cv >= 1024 ? 1024 : (cv + 63) / 64 * 64;
+    const int cv = D / (wide ? 8 : 4);
+    const bool few = frames < device_cu_count(current_device()) && tokens_per_frame >= 8 && cv > 64;
+    const int threads = few ? 64 : cv >= 1024 ? 1024 : (cv + 63) / 64 * 64;
+    const dim3 grid(frames, few ? ceil_div(cv, 64) : 1);
+    hipStream_t s = (hipStream_t)stream;
     with_dtype(h_dtype, [&](auto ti) {
         typedef decltype(ti) T;
-        if (wide) hipLaunchKernelGGL((pool_score_save_kernel<T, 8>), dim3(frames), dim3(threads), 0, (hipStream_t)stream, (const T*)h, ldh, tokens_per_frame, cv, w, b, logits, pooled, ldp);
-        else hipLaunchKernelGGL((pool_score_save_kernel<T, 4>), dim3(frames), dim3(threads), 0, (hipStream_t)stream, (const T*)h, ldh, tokens_per_frame, cv, w, b, logits, pooled, ldp);
+        auto run = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(threads), 0, s, (const T*)h, ldh, tokens_per_frame, cv, w, b, logits, pooled, ldp); };
+        if (few) { if (wide) run(pool_score_save_kernel<T, 8, false>); else run(pool_score_save_kernel<T, 4, false>); }
+        else if (wide) run(pool_score_save_kernel<T, 8, true>);
+        else run(pool_score_save_kernel<T, 4, true>);
     });
+    if (few) hipLaunchKernelGGL(pool_dot_kernel, dim3(frames), dim3(256), 0, s, pooled, ldp, D, w, b, logits);
     return launched();
 }
 

@@ -604,43 +604,62 @@ def attention_split(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: torch.
 # ---- training operators (csrc/train_embed.hip, train_head.hip, train_clip.hip, swiglu.hip) -------------------------------------------------------
 # Every tensor of a call lives on one device, and the call runs on that device's current stream.  A workspace that is not given is allocated for the call
 # from torch's caching allocator; a given one belongs to the call until it has run (two captured graphs that may replay at the same time need one each).
+# The checks read each tensor's attributes once and pass plain integers on: a call on a small tensor is mostly this file's time.
 _FLOATS = (torch.bfloat16, torch.float16, torch.float32)
+_HALVES = (torch.bfloat16, torch.float16)
+_SIZE = {torch.bfloat16: 2, torch.float16: 2, torch.float32: 4, torch.int64: 8}
+_raw_stream = torch._C._cuda_getCurrentRawStream
 
 
 def _fail(msg: str):
     raise _lib.VitgError(msg)
 
 
-def _same_device(*tensors: Optional[torch.Tensor]) -> torch.device:
-    """the one device that all given tensors live on"""
-    dev = None
+def _same_device(*tensors: Optional[torch.Tensor]) -> int:
+    """the index of the one device that all given tensors live on"""
+    idx = None
     for t in tensors:
         if t is None:
             continue
-        _req(t)
-        if dev is not None and t.device != dev:
-            _fail(f"tensors on {dev} and {t.device}: one call works on one device")
-        dev = t.device
-    return dev
+        i = t.get_device()
+        if i < 0:
+            _req(t)
+        if idx is None:
+            idx = i
+        elif i != idx:
+            _fail(f"tensors on cuda:{idx} and cuda:{i}: one call works on one device")
+    return idx
 
 
-def _matrix(t: torch.Tensor, what: str, rows: int, cols: int, dtypes, ld_multiple: int = 1) -> int:
-    """checks a [rows, cols] matrix with unit column stride and rows that do not overlap; returns its leading dimension"""
-    if t.dtype not in dtypes:
-        _fail(f"{what}: expected one of {tuple(str(d) for d in dtypes)}, got {t.dtype}")
-    if t.dim() != 2 or t.shape[0] != rows or t.shape[1] != cols:
-        _fail(f"{what}: expected [{rows}, {cols}], got {tuple(t.shape)}")
-    if rows >= 1 << 31 or cols >= 1 << 31 or t.stride(0) >= 1 << 31:
-        _fail(f"{what}: sizes and row strides below 2^31 required")
-    if rows * cols == 0:
-        return max(cols, ld_multiple)
-    if cols > 1 and t.stride(1) != 1:
+def _call_on(idx: int, name: str, *args) -> None:
+    """the entry point on device idx and its current stream (the last argument)"""
+    if torch.cuda.current_device() == idx:
+        _lib.check(getattr(_lib.load(), name)(*args, _raw_stream(idx)), name)
+    else:
+        with torch.cuda.device(idx):
+            _lib.check(getattr(_lib.load(), name)(*args, _raw_stream(idx)), name)
+
+
+def _matrix(t: torch.Tensor, what: str, rows: int, cols: int, dtypes):
+    """checks a [rows, cols] matrix with unit column stride and rows that do not overlap -> (address, leading dimension, end address)"""
+    dt, shape = t.dtype, t.shape
+    if dt not in dtypes:
+        _fail(f"{what}: expected one of {tuple(str(d) for d in dtypes)}, got {dt}")
+    if len(shape) != 2 or shape[0] != rows or shape[1] != cols:
+        _fail(f"{what}: expected [{rows}, {cols}], got {tuple(shape)}")
+    ptr = t.data_ptr()
+    if rows == 0 or cols == 0:
+        return ptr, (cols + 7) & -8, ptr
+    ld, step = t.stride()
+    if step != 1 and cols > 1:
         _fail(f"{what}: unit column stride required")
     if rows == 1:                                        # (the stride of a size-1 dimension is arbitrary in torch)
-        return -(-cols // ld_multiple) * ld_multiple
-    if t.stride(0) < cols:
-        _fail(f"{what}: rows overlap (row stride {t.stride(0)} < {cols})")
-    return t.stride(0)
+        ld = (cols + 7) & -8
+    elif ld < cols:
+        _fail(f"{what}: rows overlap (row stride {ld} < {cols})")
+    if (rows | cols | ld) >> 31:
+        _fail(f"{what}: sizes and row strides below 2^31 required")
+    return ptr, ld, ptr + ((rows - 1) * ld + cols) * _SIZE[dt]
 
 
 def _shape2(t: torch.Tensor, what: str):
@@ -649,54 +668,48 @@ def _shape2(t: torch.Tensor, what: str):
     return t.shape
 
 
-def _vector(t: torch.Tensor, what: str, n: int, dtype: torch.dtype) -> torch.Tensor:
+def _vector(t: torch.Tensor, what: str, n: int, dtype: torch.dtype):
+    """checks n contiguous values -> (address, end address)"""
     if t.dtype != dtype or t.numel() != n or not t.is_contiguous():
         _fail(f"{what}: expected {n} contiguous values of {dtype}, got {tuple(t.shape)} of {t.dtype}")
-    return t
+    ptr = t.data_ptr()
+    return ptr, ptr + n * _SIZE[dtype]
 
 
-def _workspace(workspace: Optional[torch.Tensor], need: int, device: torch.device) -> torch.Tensor:
+def _workspace(workspace: Optional[torch.Tensor], need: int, idx: int):
+    """-> (tensor, address, bytes) of at least `need` bytes"""
     if workspace is None:
-        return torch.empty(max(need, 16), dtype=torch.uint8, device=device)
-    if workspace.device != device or not workspace.is_contiguous():
-        _fail("workspace: contiguous and on the call's device")
-    if workspace.numel() * workspace.element_size() < need:
-        _fail(f"workspace: {workspace.numel() * workspace.element_size()} bytes given, {need} needed")
-    return workspace
+        ws = torch.empty(need if need > 16 else 16, dtype=torch.uint8, device=idx)
+        return ws, ws.data_ptr(), ws.numel()
+    if not workspace.is_contiguous():
+        _fail("workspace: contiguous memory required")
+    have = workspace.numel() * workspace.element_size()
+    if have < need:
+        _fail(f"workspace: {have} bytes given, {need} needed")
+    return workspace, workspace.data_ptr(), have
 
 
-def _overlap(a: Optional[torch.Tensor], b: Optional[torch.Tensor]) -> bool:
-    """whether the memory ranges that two tensors span meet"""
-    if a is None or b is None or a.numel() == 0 or b.numel() == 0:
-        return False
-
-    def span(t):
-        last = sum((n - 1) * st for n, st in zip(t.shape, t.stride()))
-        return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
-    (a0, a1), (b0, b1) = span(a), span(b)
-    return a0 < b1 and b0 < a1
-
-
-def _distinct(outputs, inputs):
-    """no output of a call shares memory with an input or another output"""
-    outs = [(n, t) for n, t in outputs if t is not None]
-    for i, (n, t) in enumerate(outs):
-        for m, u in outs[i + 1:] + [(m, u) for m, u in inputs if u is not None]:
-            if _overlap(t, u):
+def _distinct(outputs, inputs=()):
+    """no output of a call shares memory with an input or another output; items are (name, address, end)"""
+    for i, (n, a, z) in enumerate(outputs):
+        for m, b, y in outputs[i + 1:]:
+            if a < y and b < z:
+                _fail(f"{n} and {m} share memory")
+        for m, b, y in inputs:
+            if a < y and b < z:
                 _fail(f"{n} and {m} share memory")
 
 
 def embed_lookup(ids: torch.Tensor, table: torch.Tensor, out: torch.Tensor, *, scale: float = 1.0) -> torch.Tensor:
     """out[i] = scale * table[ids[i]] (fp32 / fp16 / bf16 table and out, one rounding); ids outside [0, vocab) - image slots, padding - give zero rows
     (vitg_embed_lookup)"""
-    dev = _same_device(ids, table, out)
+    idx = _same_device(ids, table, out)
     n, (vocab, d) = ids.numel(), _shape2(table, "table")
-    _vector(ids, "ids", n, torch.int64)
-    ldt = _matrix(table, "table", vocab, d, _FLOATS, 8)
-    ldo = _matrix(out, "out", n, d, _FLOATS, 8)
-    _distinct([("out", out)], [("table", table), ("ids", ids)])
-    with torch.cuda.device(dev):
-        _lib.call("vitg_embed_lookup", _ptr(ids), n, _ptr(table), dt_code(table.dtype), ldt, vocab, d, float(scale), _ptr(out), dt_code(out.dtype), ldo, _stream())
+    pi, ei = _vector(ids, "ids", n, torch.int64)
+    pt, ldt, et = _matrix(table, "table", vocab, d, _FLOATS)
+    po, ldo, eo = _matrix(out, "out", n, d, _FLOATS)
+    _distinct([("out", po, eo)], [("table", pt, et), ("ids", pi, ei)])
+    _call_on(idx, "vitg_embed_lookup", pi, n, pt, _DT[table.dtype], ldt, vocab, d, scale, po, _DT[out.dtype], ldo)
     return out
 
 
@@ -711,35 +724,32 @@ def embed_backward(ids: torch.Tensor, dout: torch.Tensor, dtable: torch.Tensor, 
                    workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
     """dtable[v] = scale * sum of dout[i] over ids[i] = v, for every row v (zero where no token is); accumulate: added to the rows of the batch, the others
     untouched.  ids outside the vocabulary contribute nothing.  Sorted tokens, fp32 sums in a fixed order (vitg_embed_backward)"""
-    dev = _same_device(ids, dout, dtable, workspace)
+    idx = _same_device(ids, dout, dtable, workspace)
     n, (vocab, d) = ids.numel(), _shape2(dtable, "dtable")
-    _vector(ids, "ids", n, torch.int64)
-    ldd = _matrix(dout, "dout", n, d, _FLOATS, 8)
-    ldt = _matrix(dtable, "dtable", vocab, d, _FLOATS, 8)
-    _distinct([("dtable", dtable)], [("dout", dout), ("ids", ids)])
-    with torch.cuda.device(dev):
-        ws = _workspace(workspace, embed_backward_plan(n, d), dev)
-        _distinct([("workspace", ws)], [("dtable", dtable), ("dout", dout), ("ids", ids)])
-        _lib.call("vitg_embed_backward", _ptr(ids), n, _ptr(dout), dt_code(dout.dtype), ldd, vocab, d, float(scale), _ptr(dtable), dt_code(dtable.dtype), ldt,
-                  int(bool(accumulate)), _ptr(ws), ws.numel() * ws.element_size(), _stream())
+    pi, ei = _vector(ids, "ids", n, torch.int64)
+    pd, ldd, ed = _matrix(dout, "dout", n, d, _FLOATS)
+    pt, ldt, et = _matrix(dtable, "dtable", vocab, d, _FLOATS)
+    ws, pw, nw = _workspace(workspace, embed_backward_plan(n, d), idx)
+    _distinct([("dtable", pt, et), ("workspace", pw, pw + nw)], [("dout", pd, ed), ("ids", pi, ei)])
+    _call_on(idx, "vitg_embed_backward", pi, n, pd, _DT[dout.dtype], ldd, vocab, d, scale, pt, _DT[dtable.dtype], ldt, 1 if accumulate else 0, pw, nw)
     return dtable
-
-
-_HALVES = (torch.bfloat16, torch.float16)
 
 
 def swiglu(x: torch.Tensor, w: torch.Tensor, out: torch.Tensor, *, gu: Optional[torch.Tensor] = None) -> torch.Tensor:
     """out = silu(x @ w_gate.T) * (x @ w_up.T), the rows of w interleaved [32 gate | 32 up] (PackedWeights' gu_w); gu [M, N]: the 16-bit pre-activations in
     that order, kept for swiglu_backward (vitg_swiglu)"""
-    dev = _same_device(x, w, out, gu)
+    idx = _same_device(x, w, out, gu)
     (m, k), nn = _shape2(x, "x"), _shape2(w, "w")[0]
-    ldx = _matrix(x, "x", m, k, _HALVES, 8)
-    ldw = _matrix(w, "w", nn, k, (x.dtype,), 8)
-    ldo = _matrix(out, "out", m, nn // 2, (x.dtype,), 8)
-    ldgu = 0 if gu is None else _matrix(gu, "gu", m, nn, (x.dtype,), 8)
-    _distinct([("out", out), ("gu", gu)], [("x", x), ("w", w)])
-    with torch.cuda.device(dev):
-        _lib.call("vitg_swiglu", _ptr(x), ldx, _ptr(w), ldw, m, nn, k, dt_code(x.dtype), _ptr(out), ldo, _ptr(gu), ldgu, _stream())
+    dt = x.dtype
+    px, ldx, ex = _matrix(x, "x", m, k, _HALVES)
+    pw, ldw, ew = _matrix(w, "w", nn, k, (dt,))
+    po, ldo, eo = _matrix(out, "out", m, nn // 2, (dt,))
+    outs, pg, ldg = [("out", po, eo)], 0, 0
+    if gu is not None:
+        pg, ldg, eg = _matrix(gu, "gu", m, nn, (dt,))
+        outs.append(("gu", pg, eg))
+    _distinct(outs, (("x", px, ex), ("w", pw, ew)))
+    _call_on(idx, "vitg_swiglu", px, ldx, pw, ldw, m, nn, k, _DT[dt], po, ldo, pg, ldg)
     return out
 
 
@@ -754,53 +764,59 @@ def swiglu_backward(dout: torch.Tensor, gu: torch.Tensor, x: torch.Tensor, w: to
                     dw: Optional[torch.Tensor] = None, accumulate: bool = False, workspace: Optional[torch.Tensor] = None) -> None:
     """gradients of swiglu(x, w, gu=gu) for dout = dL/d out: dx (overwritten) and dw (x's type or fp32; accumulate adds to what it holds).  Either may be
     left out (vitg_swiglu_backward)"""
-    dev = _same_device(dout, gu, x, w, dx, dw, workspace)
+    idx = _same_device(dout, gu, x, w, dx, dw, workspace)
     (m, k), nn = _shape2(x, "x"), _shape2(w, "w")[0]
-    ldx = _matrix(x, "x", m, k, _HALVES, 8)
-    ldw = _matrix(w, "w", nn, k, (x.dtype,), 8)
-    lddo = _matrix(dout, "dout", m, nn // 2, (x.dtype,), 8)
-    ldgu = _matrix(gu, "gu", m, nn, (x.dtype,), 8)
-    lddx = 0 if dx is None else _matrix(dx, "dx", m, k, (x.dtype,), 8)
-    lddw = 0 if dw is None else _matrix(dw, "dw", nn, k, (x.dtype, torch.float32), 8)
-    ins = [("dout", dout), ("gu", gu), ("x", x), ("w", w)]
-    _distinct([("dx", dx), ("dw", dw)], ins)
-    if dx is None and dw is None:
+    dt = x.dtype
+    px, ldx, ex = _matrix(x, "x", m, k, _HALVES)
+    pw, ldw, ew = _matrix(w, "w", nn, k, (dt,))
+    pd, ldd, ed = _matrix(dout, "dout", m, nn // 2, (dt,))
+    pg, ldg, eg = _matrix(gu, "gu", m, nn, (dt,))
+    outs, pdx, lddx, pdw, lddw, dwt = [], 0, 0, 0, 0, dt
+    if dx is not None:
+        pdx, lddx, e = _matrix(dx, "dx", m, k, (dt,))
+        outs.append(("dx", pdx, e))
+    if dw is not None:
+        dwt = dw.dtype
+        pdw, lddw, e = _matrix(dw, "dw", nn, k, (dt, torch.float32))
+        outs.append(("dw", pdw, e))
+    if not outs:
         return
-    with torch.cuda.device(dev):
-        ws = _workspace(workspace, swiglu_backward_plan(m, nn, k, dx is not None, dw is not None), dev)
-        _distinct([("workspace", ws)], ins + [("dx", dx), ("dw", dw)])
-        _lib.call("vitg_swiglu_backward", _ptr(dout), lddo, _ptr(gu), ldgu, _ptr(x), ldx, _ptr(w), ldw, m, nn, k, dt_code(x.dtype), _ptr(dx), lddx, _ptr(dw),
-                  lddw, dt_code(x.dtype if dw is None else dw.dtype), int(bool(accumulate)), _ptr(ws), ws.numel() * ws.element_size(), _stream())
+    ws, pws, nws = _workspace(workspace, swiglu_backward_plan(m, nn, k, dx is not None, dw is not None), idx)
+    outs.append(("workspace", pws, pws + nws))
+    _distinct(outs, (("dout", pd, ed), ("gu", pg, eg), ("x", px, ex), ("w", pw, ew)))
+    _call_on(idx, "vitg_swiglu_backward", pd, ldd, pg, ldg, px, ldx, pw, ldw, m, nn, k, _DT[dt], pdx, lddx, pdw, lddw, _DT[dwt], 1 if accumulate else 0, pws, nws)
 
 
 def pool_score_save(h: torch.Tensor, frames: int, tokens_per_frame: int, d: int, w: torch.Tensor, b: torch.Tensor, logits: torch.Tensor,
                     pooled: torch.Tensor) -> torch.Tensor:
     """pool_score on fp32 / fp16 / bf16 rows that keeps the frame means pooled [frames, d] (fp32) for pool_score_backward (vitg_pool_score_save)"""
-    dev = _same_device(h, w, b, logits, pooled)
+    idx = _same_device(h, w, b, logits, pooled)
     if tokens_per_frame <= 0 or frames < 0:
         _fail("frames >= 0 and tokens_per_frame >= 1 required")
-    ldh = _matrix(h, "h", frames * tokens_per_frame, d, _FLOATS, 8)
-    ldp = _matrix(pooled, "pooled", frames, d, (torch.float32,), 4)
-    _vector(w, "w", d, torch.float32); _vector(b, "b", 1, torch.float32); _vector(logits, "logits", frames, torch.float32)
-    _distinct([("logits", logits), ("pooled", pooled)], [("h", h), ("w", w), ("b", b)])
-    with torch.cuda.device(dev):
-        _lib.call("vitg_pool_score_save", _ptr(h), dt_code(h.dtype), ldh, frames, tokens_per_frame, d, _ptr(w), _ptr(b), _ptr(logits), _ptr(pooled), ldp, _stream())
+    ph, ldh, eh = _matrix(h, "h", frames * tokens_per_frame, d, _FLOATS)
+    pp, ldp, ep = _matrix(pooled, "pooled", frames, d, (torch.float32,))
+    (pw, ew), (pb, eb), (pl, el) = _vector(w, "w", d, torch.float32), _vector(b, "b", 1, torch.float32), _vector(logits, "logits", frames, torch.float32)
+    _distinct([("logits", pl, el), ("pooled", pp, ep)], (("h", ph, eh), ("w", pw, ew), ("b", pb, eb)))
+    _call_on(idx, "vitg_pool_score_save", ph, _DT[h.dtype], ldh, frames, tokens_per_frame, d, pw, pb, pl, pp, ldp)
     return logits
 
 
 def bce_loss_backward(logits: torch.Tensor, labels: torch.Tensor, *, scale: float = 1.0):
     """-> (loss, pos_weight, dlogits): bce_loss and scale * d loss / d logits (vitg_bce_loss_backward)"""
-    dev = _same_device(logits, labels)
-    _req(logits, torch.float32)
-    _req(labels, torch.float32)
-    if logits.numel() != labels.numel() or logits.numel() == 0:
+    idx = _same_device(logits, labels)
+    n = logits.numel()
+    if logits.dtype != torch.float32 or labels.dtype != torch.float32:
+        _fail(f"logits and labels must be fp32, got {logits.dtype} and {labels.dtype}")
+    if n != labels.numel() or n == 0:
         _fail("logits and labels must have the same, non-zero, number of elements")
-    with torch.cuda.device(dev):
-        z, y = logits.contiguous(), labels.contiguous()
-        out = torch.empty(2, dtype=torch.float32, device=dev)
-        dz = torch.empty(z.shape, dtype=torch.float32, device=dev)
-        _lib.call("vitg_bce_loss_backward", _ptr(z), _ptr(y), z.numel(), float(scale), _ptr(out), _ptr(dz), _stream())
-    return out[0], out[1], dz
+    if n >> 31:
+        _fail("fewer than 2^31 logits required")
+    z, y = logits.contiguous(), labels.contiguous()
+    out = torch.empty(2, dtype=torch.float32, device=idx)
+    dz = torch.empty(logits.shape, dtype=torch.float32, device=idx)
+    _call_on(idx, "vitg_bce_loss_backward", z.data_ptr(), y.data_ptr(), n, scale, out.data_ptr(), dz.data_ptr())
+    loss, weight = out.unbind(0)
+    return loss, weight, dz
 
 
 def pool_score_backward(pooled: torch.Tensor, frames: int, tokens_per_frame: int, d: int, w: torch.Tensor, dlogits: torch.Tensor,
@@ -808,39 +824,24 @@ def pool_score_backward(pooled: torch.Tensor, frames: int, tokens_per_frame: int
                         accumulate: bool = False) -> None:
     """gradients of pool_score_save: dh [frames * tokens_per_frame, d] (fp32 / fp16 / bf16, overwritten), dw [d] and db [1] (fp32; accumulate adds to what they
     hold) - each may be left out (vitg_pool_score_backward)"""
-    dev = _same_device(pooled, w, dlogits, dh, dw, db)
+    idx = _same_device(pooled, w, dlogits, dh, dw, db)
     if tokens_per_frame <= 0 or frames < 0:
         _fail("frames >= 0 and tokens_per_frame >= 1 required")
-    ldp = _matrix(pooled, "pooled", frames, d, (torch.float32,), 4)
-    lddh = 0 if dh is None else _matrix(dh, "dh", frames * tokens_per_frame, d, _FLOATS, 8)
-    _vector(w, "w", d, torch.float32); _vector(dlogits, "dlogits", frames, torch.float32)
+    pp, ldp, ep = _matrix(pooled, "pooled", frames, d, (torch.float32,))
+    (pw, ew), (pz, ez) = _vector(w, "w", d, torch.float32), _vector(dlogits, "dlogits", frames, torch.float32)
+    outs, ph, ldh, hdt, pdw, pdb = [], 0, 0, torch.float32, 0, 0
+    if dh is not None:
+        hdt = dh.dtype
+        ph, ldh, e = _matrix(dh, "dh", frames * tokens_per_frame, d, _FLOATS)
+        outs.append(("dh", ph, e))
     if dw is not None:
-        _vector(dw, "dw", d, torch.float32)
+        pdw, e = _vector(dw, "dw", d, torch.float32)
+        outs.append(("dw", pdw, e))
     if db is not None:
-        _vector(db, "db", 1, torch.float32)
-    _distinct([("dh", dh), ("dw", dw), ("db", db)], [("pooled", pooled), ("w", w), ("dlogits", dlogits)])
-    with torch.cuda.device(dev):
-        _lib.call("vitg_pool_score_backward", _ptr(pooled), ldp, frames, tokens_per_frame, d, _ptr(w), _ptr(dlogits), _ptr(dh),
-                  dt_code(torch.float32 if dh is None else dh.dtype), lddh, _ptr(dw), _ptr(db), int(bool(accumulate)), _stream())
-
-
-def _grad_arrays(grads, outs):
-    n = len(grads)
-    for i, t in enumerate(grads):
-        _req(t)
-        if t.dtype not in _FLOATS:
-            _fail(f"gradient {i}: fp32, fp16 or bf16 expected, got {t.dtype}")
-        if not t.is_contiguous():
-            _fail(f"gradient {i}: contiguous tensors only")
-    if outs is not None:
-        if len(outs) != n:
-            _fail(f"{n} gradients and {len(outs)} outputs")
-        for i, (t, o) in enumerate(zip(grads, outs)):
-            if o.dtype != t.dtype or o.numel() != t.numel() or not o.is_contiguous():
-                _fail(f"output {i}: a contiguous tensor of the gradient's type and size required")
-    numel = (C.c_long * n)(*[t.numel() for t in grads])
-    dtype = (C.c_int * n)(*[dt_code(t.dtype) for t in grads])
-    return n, numel, dtype
+        pdb, e = _vector(db, "db", 1, torch.float32)
+        outs.append(("db", pdb, e))
+    _distinct(outs, (("pooled", pp, ep), ("w", pw, ew), ("dlogits", pz, ez)))
+    _call_on(idx, "vitg_pool_score_backward", pp, ldp, frames, tokens_per_frame, d, pw, pz, ph, _DT[hdt], ldh, pdw, pdb, 1 if accumulate else 0)
 
 
 def clip_grad_norm(grads, max_norm: Optional[float], *, outs=None, scale: float = 1.0, norm: Optional[torch.Tensor] = None,
@@ -849,37 +850,44 @@ def clip_grad_norm(grads, max_norm: Optional[float], *, outs=None, scale: float 
     or in `outs`.  max_norm None: the norm alone, nothing is written.  scale: 1 / loss scale.  Nothing is read back to the host; an infinite or NaN norm shows
     in the norm (vitg_clip_grad)"""
     grads = list(grads)
-    if not grads:
+    n = len(grads)
+    if not n:
         _fail("no gradients: at least one tensor (it may be empty) names the device")
-    outs = None if outs is None else list(outs)
-    if max_norm is None and outs is not None:
-        _fail("max_norm None computes the norm alone: no outs")
-    if max_norm is not None and not float(max_norm) >= 0.0:
+    if max_norm is None:
+        if outs is not None:
+            _fail("max_norm None computes the norm alone: no outs")
+    elif not float(max_norm) >= 0.0:
         _fail(f"max_norm must not be negative, got {max_norm}")
-    n, numel, dtype = _grad_arrays(grads, outs)
-    dev = _same_device(*grads, *(outs or []), norm, workspace)
-    if norm is not None:
-        _vector(norm, "norm", 1, torch.float32)
-    if max_norm is not None:
-        # every output is its own gradient or memory of its own: a shared byte would be scaled twice, or before another block has read it
-        spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size(), k) for k, t in
-                       [(2 * i, t) for i, t in enumerate(grads)] + [(2 * i + 1, o) for i, o in enumerate(outs or [])
-                                                                    if o.data_ptr() != grads[i].data_ptr()] if t.numel())
-        written = lambda k: outs is None or k & 1 or outs[k // 2].data_ptr() == grads[k // 2].data_ptr()        # noqa: E731
-        end, last = 0, None
-        for a, z, k in spans:
-            if a < end and (written(k) or written(last)):
-                _fail("two of the call's tensors share memory, and one of them is written")
-            if z > end:
-                end, last = z, k
-    with torch.cuda.device(dev):
-        if norm is None:
-            norm = torch.empty(1, dtype=torch.float32, device=dev)
-        need = C.c_long(0)
-        _lib.call("vitg_clip_grad_plan", n, numel, dtype, C.byref(need))
-        ws = _workspace(workspace, need.value, dev)
-        pin = (C.c_void_p * n)(*[t.data_ptr() for t in grads])
-        pout = None if max_norm is None else (C.c_void_p * n)(*[t.data_ptr() for t in (outs if outs is not None else grads)])
-        _lib.call("vitg_clip_grad", n, pin, pout, numel, dtype, float(scale), 0.0 if max_norm is None else float(max_norm), _ptr(norm), _ptr(ws),
-                  ws.numel() * ws.element_size(), _stream())
+    idx = _same_device(*grads, norm, workspace)
+    numel, codes, pin = [], [], []
+    for t in grads:
+        code = _DT.get(t.dtype)
+        if code is None or not t.is_contiguous():
+            _fail(f"gradients: contiguous tensors of fp32, fp16 or bf16, got {tuple(t.shape)} of {t.dtype}, strides {t.stride()}")
+        codes.append(code)
+        numel.append(t.numel())
+        pin.append(t.data_ptr())
+    pout = None
+    if outs is not None:
+        outs = list(outs)
+        if len(outs) != n:
+            _fail(f"{n} gradients and {len(outs)} outputs")
+        _same_device(grads[0], *outs)
+        pout = []
+        for t, o, k in zip(grads, outs, numel):
+            if o.dtype != t.dtype or o.numel() != k or not o.is_contiguous():
+                _fail("outs: contiguous tensors of the gradients' types and sizes required")
+            pout.append(o.data_ptr())
+    elif max_norm is not None:
+        pout = pin
+    if norm is None:
+        norm = torch.empty(1, dtype=torch.float32, device=idx)
+    pn, en = _vector(norm, "norm", 1, torch.float32)
+    longs, pointers = C.c_long * n, C.c_void_p * n
+    numel, codes, need = longs(*numel), (C.c_int * n)(*codes), C.c_long(0)
+    _lib.call("vitg_clip_grad_plan", n, numel, codes, C.byref(need))
+    ws, pw, nw = _workspace(workspace, need.value, idx)
+    _distinct([("norm", pn, en), ("workspace", pw, pw + nw)])
+    _call_on(idx, "vitg_clip_grad", n, pointers(*pin), None if pout is None else pointers(*pout), numel, codes, scale, 0.0 if max_norm is None else max_norm,
+             pn, pw, nw)
     return norm
