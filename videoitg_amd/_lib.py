@@ -82,8 +82,8 @@ SIGNATURES = {
     "vitg_pool_score_save": [_p, _i, _l, _i, _i, _i, _p, _p, _p, _p, _l, _p],
     "vitg_bce_loss_backward": [_p, _p, _i, _f, _p, _p, _p],
     "vitg_pool_score_backward": [_p, _l, _i, _i, _i, _p, _p, _p, _i, _l, _p, _p, _i, _p],
-    "vitg_clip_grad_plan": [_i, C.POINTER(C.c_long), C.POINTER(C.c_int), C.POINTER(C.c_long)],
-    "vitg_clip_grad": [_i, C.POINTER(C.c_void_p), C.POINTER(C.c_void_p), C.POINTER(C.c_long), C.POINTER(C.c_int), _f, _f, _p, _p, _l, _p],
+    "vitg_clip_grad_plan": [_i, _p, _p, C.POINTER(C.c_long)],
+    "vitg_clip_grad": [_i, _p, _p, _p, _p, _f, _f, _p, _p, _l, _p],          # (host arrays: addresses, sizes, dtype codes)
     "vitg_attention_split": [_p, _p, _p, _p, _l, _l, _l, _l, _i, _i, _i, _i, _i, _i, _l, _l, _l, _l, _i, _i, _i, _i, _i, _i, _i, _i, _f, _p],
 }
 

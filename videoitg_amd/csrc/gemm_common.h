@@ -316,6 +316,8 @@ int gemm256_pick_cfg(const GemmArgs& g, int mode);                              
 int gemm256_norm_cols(const GemmArgs& g);                                       // gemm256.hip
 int launch_gemm_mi16_streamk(const GemmArgs& g, int dtype, int blocks, hipStream_t s);   // gemm_mi16.hip: raw fp32 partial tiles of a stream-K partition
 int launch_gemm128_swiglu(GemmArgs g, int dtype, hipStream_t s);                        // gemm.hip: the 128x128 tile's SwiGLU, with g.gu its pre-activations too
+int launch_gemm_ring(const GemmArgs& g, int dtype, int mode, bool kmajor, hipStream_t s);  // gemm_ring.hip: at most one 128x128 tile per CU
+int launch_gemm_ring_pair(const GemmArgs& kmajor, const GemmArgs& nt, int dtype, hipStream_t s);
 int launch_gemm_mi16_kmajor(const GemmArgs& g, int dtype, int bm, hipStream_t s);         // gemm_mi16.hip: the weight operand as W[K, N]
 int launch_gemm_mi16_swiglu_save(const GemmArgs& g, int dtype, hipStream_t s);          // gemm_mi16.hip: MODE_SWIGLU that stores its pre-activations too
 int launch_gemm_mi16(const GemmArgs& g, int dtype, int mode, int cfg, hipStream_t s);   // gemm_mi16.hip: the same tiles on v_mfma_f32_16x16x32

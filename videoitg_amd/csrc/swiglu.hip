@@ -16,11 +16,8 @@ namespace vitg {
 // out[c, r] = in[r, c] for r < R, c < C; columns R .. Rp-1 of out are zero (K padding of the GEMM that reads it).  64 x 64 tiles through LDS.
 constexpr int TR_LD = 72;                                // halfs per LDS row: 16-B aligned
 template <typename T>
-__global__ __launch_bounds__(256) void transpose16_kernel(const T* __restrict__ in, long ldi, long R, int C, T* __restrict__ out, long ldo, long Rp) {
-    typedef typename T16<T>::vec8 vec8;
-    __shared__ __attribute__((aligned(16))) T tile[64 * TR_LD];          // [c][r]
-    const long r0 = (long)blockIdx.x * 64;
-    const int c0 = blockIdx.y * 64;
+__device__ __forceinline__ void transpose_tile(T* tile, long r0, int c0, const T* __restrict__ in, long ldi, long R, int C, T* __restrict__ out, long ldo, long Rp) {
+    typedef typename T16<T>::vec8 vec8;                  // tile: [c][r]
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
         const int idx = i * 256 + threadIdx.x, r = idx >> 3, cq = (idx & 7) * 8;
@@ -42,12 +39,10 @@ __global__ __launch_bounds__(256) void transpose16_kernel(const T* __restrict__ 
 // dGU from dH and the saved pre-activations, in both orders: dgu [M, 2F] (unless null) and dgut [2F, Mp] (unless null; columns M .. Mp-1 zero).
 // One block: 64 rows x 32 features = 64 columns of gu.
 template <typename T>
-__global__ __launch_bounds__(256) void swiglu_grad_kernel(const T* __restrict__ dh, long lddh, const T* __restrict__ gu, long ldgu, long M, long Mp,
-                                                          T* __restrict__ dgu, long lddgu, T* __restrict__ dgut) {
-    typedef typename T16<T>::vec8 vec8;
-    __shared__ __attribute__((aligned(16))) T tile[64 * TR_LD];          // [column of gu][row]
-    const long r0 = (long)blockIdx.x * 64;
-    const int f0 = blockIdx.y * 32, n0 = blockIdx.y * 64;
+__device__ __forceinline__ void swiglu_grad_tile(T* tile, long r0, int n0, const T* __restrict__ dh, long lddh, const T* __restrict__ gu, long ldgu, long M, long Mp,
+                                                 T* __restrict__ dgu, long lddgu, T* __restrict__ dgut) {
+    typedef typename T16<T>::vec8 vec8;                  // tile: [column of gu][row]
+    const int f0 = n0 / 2;
     {
         const int r = threadIdx.x >> 2, q = (threadIdx.x & 3) * 8;
         const long m = r0 + r;
@@ -81,6 +76,22 @@ __global__ __launch_bounds__(256) void swiglu_grad_kernel(const T* __restrict__ 
         const int idx = i * 256 + threadIdx.x, c = idx >> 3, rq = (idx & 7) * 8;
         *(vec8*)(dgut + (long)(n0 + c) * Mp + r0 + rq) = *(const vec8*)(tile + c * TR_LD + rq);
     }
+}
+
+// everything in front of the products in one launch: blocks [0, grad) dGU, then the tiles of X^T [K, Mp], then those of W^T [K, N] (64 x 64 each)
+template <typename T>
+struct SwigluPrep {
+    const T* dh; long lddh; const T* gu; long ldgu; long M, Mp; T* dgu; long lddgu; T* dgut;
+    const T* x; long ldx; T* xt; const T* w; long ldw; T* wt;
+    int N, K; long grad, x_end;
+};
+template <typename T>
+__global__ __launch_bounds__(256) void swiglu_prep_kernel(const SwigluPrep<T> a) {
+    __shared__ __attribute__((aligned(16))) T tile[64 * TR_LD];
+    const long mt = a.Mp / 64, id = blockIdx.x;
+    if (id < a.grad) swiglu_grad_tile<T>(tile, id % mt * 64, (int)(id / mt) * 64, a.dh, a.lddh, a.gu, a.ldgu, a.M, a.Mp, a.dgu, a.lddgu, a.dgut);
+    else if (id < a.x_end) transpose_tile<T>(tile, (id - a.grad) % mt * 64, (int)((id - a.grad) / mt) * 64, a.x, a.ldx, a.M, a.K, a.xt, a.Mp, a.Mp);
+    else transpose_tile<T>(tile, (id - a.x_end) % (a.N / 64) * 64, (int)((id - a.x_end) / (a.N / 64)) * 64, a.w, a.ldw, a.N, a.K, a.wt, a.N, a.N);
 }
 
 // rows of `bytes` (a multiple of 16) set to zero, `pitch` bytes apart
@@ -166,14 +177,14 @@ template <typename V8> __device__ __forceinline__ void transpose8(const V8 (&in)
 // it in registers into 8 MFMA operands - column d0 + 8 (lane & 15) + j of W is row (lane & 15) of operand j, so a lane's 8 accumulators are 32 consecutive
 // columns of dX.  A block: 128 columns x one share of the rows, split over four waves, summed as (w0 + w2) + (w1 + w3) into part[share][m][K] (fp32).
 template <typename T, int MT>
-__global__ __launch_bounds__(256) void swiglu_dx_rows_kernel(const T* __restrict__ dgu, long lddgu, const T* __restrict__ W, long ldw, int M, int N, int K,
-                                                             int shares, float* __restrict__ part) {
+__device__ __forceinline__ void dx_rows_block(int column, int share, const T* __restrict__ dgu, long lddgu, const T* __restrict__ W, long ldw, int M, int N, int K,
+                                              int shares, float* __restrict__ part) {
     typedef typename T16<T>::vec8 vec8;
     __shared__ __attribute__((aligned(16))) f32x4 red[2][8][64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r16 = lane & 15, q = lane >> 4;
-    const int d0 = blockIdx.x * 128;
+    const int d0 = column * 128;
     const int col = min(d0 + ((r16 & 3) * 4 + (r16 >> 2)) * 8, K - 8);   // (the last block may hang over: its loads repeat, its stores are left out)
-    const long steps = N / 32, ways = (long)shares * 4, way = (long)blockIdx.y * 4 + wave;
+    const long steps = N / 32, ways = (long)shares * 4, way = (long)share * 4 + wave;
     const long s0 = steps * way / ways, s1 = steps * (way + 1) / ways;
     const T* const wp = W + (long)(q * 8) * ldw + col;
     const T* gp[MT];
@@ -219,7 +230,7 @@ __global__ __launch_bounds__(256) void swiglu_dx_rows_kernel(const T* __restrict
         if (wave != 0 || m >= M) continue;
 #pragma unroll
         for (int j = 0; j < 8; ++j) acc[i][j] += red[1][j][lane];
-        float* const o = part + ((long)blockIdx.y * M + m) * K;
+        float* const o = part + ((long)share * M + m) * K;
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             const int d = d0 + (r * 4 + q) * 8;
@@ -230,36 +241,46 @@ __global__ __launch_bounds__(256) void swiglu_dx_rows_kernel(const T* __restrict
     }
 }
 
-// out[m, :] (+)= sum of the shares [share][M][K] in order
+// out[m, :] (+)= sum of the shares [share][M][K] in order, for one or two matrices (blocks [0, a_blocks) the first)
+struct JoinArgs { const float* part; long M; int K, shares; void* out; long ldo; int accumulate; };
 template <typename T>
-__global__ __launch_bounds__(256) void join_shares_kernel(const float* __restrict__ part, long M, int K, int shares, T* __restrict__ out, long ldo, int accumulate) {
-    const long i = ((long)blockIdx.x * 256 + threadIdx.x) * 4, total = M * K;
+__device__ __forceinline__ void join_quad(const JoinArgs& a, long i) {
+    const long total = a.M * a.K;
     if (i >= total) return;
-    f32x4 v = *(const f32x4*)(part + i);
+    f32x4 v = *(const f32x4*)(a.part + i);
 #pragma unroll 8
-    for (int s = 1; s < shares; ++s) v += *(const f32x4*)(part + s * total + i);
-    T* const o = out + i / K * ldo + i % K;
+    for (int s = 1; s < a.shares; ++s) v += *(const f32x4*)(a.part + s * total + i);
+    T* const o = (T*)a.out + i / a.K * a.ldo + i % a.K;
     float w[4] = {0.f, 0.f, 0.f, 0.f};
-    if (accumulate) load_vec<T, 4>(o, w);
+    if (a.accumulate) load_vec<T, 4>(o, w);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) w[e] = accumulate ? w[e] + v[e] : v[e];
+    for (int e = 0; e < 4; ++e) w[e] = a.accumulate ? w[e] + v[e] : v[e];
     store_vec<T, 4>(o, w);
 }
-template <typename T> static void join_shares(const float* part, long M, int K, int shares, void* out, long ldo, int accumulate, hipStream_t s) {
-    hipLaunchKernelGGL(join_shares_kernel<T>, dim3((unsigned)((M * K / 4 + 255) / 256)), dim3(256), 0, s, part, M, K, shares, (T*)out, ldo, accumulate);
+template <typename TA, typename TB>
+__global__ __launch_bounds__(256) void join_shares_kernel(const JoinArgs a, int a_blocks, const JoinArgs b) {
+    if ((int)blockIdx.x < a_blocks) join_quad<TA>(a, ((long)blockIdx.x * 256 + threadIdx.x) * 4);
+    else join_quad<TB>(b, ((long)((int)blockIdx.x - a_blocks) * 256 + threadIdx.x) * 4);
+}
+template <typename TA, typename TB = TA> static void join_shares(const JoinArgs& a, hipStream_t s, const JoinArgs& b = JoinArgs{}) {
+    const int na = (int)((a.M * a.K / 4 + 255) / 256), nb = (int)((b.M * b.K / 4 + 255) / 256);
+    hipLaunchKernelGGL((join_shares_kernel<TA, TB>), dim3(na + nb), dim3(256), 0, s, a, na, b);
 }
 
-// dW (+)= dGU^T X for M <= 32 rows: a wave owns 64 rows x 128 columns of dW.  A = X transposed in registers (as above), B = dGU^T rows from the transposed copy.  Bound by the write of dW.
+// dW (+)= dGU^T X for M <= 32 rows: a wave owns 32 rows x 128 columns of dW.  A = X transposed in registers (as above), B = dGU^T rows from the transposed copy.
+// Bound by the write of dW.
+constexpr int DW_WAVE = 32;
 template <typename T, typename TW>
-__global__ __launch_bounds__(256) void swiglu_dw_rows_kernel(const T* __restrict__ dgut, long Mp, const T* __restrict__ X, long ldx, int M, int N, int K,
-                                                             TW* __restrict__ dW, long lddw, int accumulate) {
+__device__ __forceinline__ void dw_rows_block(int column, int rows, const T* __restrict__ dgut, long Mp, const T* __restrict__ X, long ldx, int M, int N, int K,
+                                              TW* __restrict__ dW, long lddw, int accumulate) {
     typedef typename T16<T>::vec8 vec8;
+    constexpr int NT = DW_WAVE / 16;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r16 = lane & 15, q = lane >> 4;
-    const long n0 = ((long)blockIdx.y * 4 + wave) * 64;
-    const int d0 = blockIdx.x * 128, col = min(d0 + ((r16 & 3) * 4 + (r16 >> 2)) * 8, K - 8);
+    const long n0 = ((long)rows * 4 + wave) * DW_WAVE;
+    const int d0 = column * 128, col = min(d0 + ((r16 & 3) * 4 + (r16 >> 2)) * 8, K - 8);
     if (n0 >= N) return;
-    f32x4 acc[4][8];
-    vec8 x[8], f[8], g[4];
+    f32x4 acc[NT][8];
+    vec8 x[8], f[8], g[NT];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         const int m = q * 8 + i;
@@ -268,14 +289,14 @@ __global__ __launch_bounds__(256) void swiglu_dw_rows_kernel(const T* __restrict
         if (m < M) x[i] = *(const vec8*)(X + (long)m * ldx + col);
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) g[i] = *(const vec8*)(dgut + (n0 + i * 16 + r16) * Mp + q * 8);
+    for (int i = 0; i < NT; ++i) g[i] = *(const vec8*)(dgut + (n0 + i * 16 + r16) * Mp + q * 8);
     transpose8(x, f);
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < NT; ++i)
 #pragma unroll
         for (int j = 0; j < 8; ++j) acc[i][j] = T16<T>::mfma16(f[j], g[i], f32x4{0.f, 0.f, 0.f, 0.f});
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < NT; ++i)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             const int d = d0 + (r * 4 + q) * 8;
@@ -289,9 +310,19 @@ __global__ __launch_bounds__(256) void swiglu_dw_rows_kernel(const T* __restrict
         }
 }
 
+// both in one launch - dX reads W while dW is written: blocks [0, dx_blocks) dX (columns fastest), the others dW
+template <typename T, typename TW, int MT>
+__global__ __launch_bounds__(256) void swiglu_rows_backward_kernel(const T* __restrict__ dgu, const T* __restrict__ W, long ldw, int M, int N, int K, int shares,
+                                                                   float* __restrict__ part, int dx_blocks, const T* __restrict__ dgut, long Mp,
+                                                                   const T* __restrict__ X, long ldx, TW* __restrict__ dW, long lddw, int accumulate) {
+    const int columns = (K + 127) / 128, id = blockIdx.x;
+    if (id < dx_blocks) dx_rows_block<T, MT>(id % columns, id / columns, dgu, N, W, ldw, M, N, K, shares, part);
+    else dw_rows_block<T, TW>((id - dx_blocks) % columns, (id - dx_blocks) / columns, dgut, Mp, X, ldx, M, N, K, dW, lddw, accumulate);
+}
+
 // rows that the three kernels take, against the GEMM forms at 3584 x 37888 (us): forward 61 - 74 at 1 - 16 rows, the 128-row tile 69 - 75 at 17 - 128;
 // dX 70 - 83 at 1 - 32, 110 at 64, the K-major GEMM 91 at 65; dW 50 at 1 - 32, the GEMM 59 - 67 with a transpose of X in front
-constexpr int FWD_ROWS = 16, DX_ROWS = 32, DW_ROWS = 32;
+constexpr int FWD_ROWS = 16, BWD_ROWS = 32;
 
 // shares of W's rows per 128 columns of dX: three blocks per CU, at least 4 steps of 32 rows per wave
 static int dx_shares(int N, int K) {
@@ -303,45 +334,54 @@ static int dx_shares(int N, int K) {
 // (12 860 rows: 2.43 + 0.12 ms against 2.78; 1 607 rows: 0.41 + 0.12 against 0.43).  Either may split its contraction (N) into fp32 partials where one round
 // of tiles leaves CUs idle.  Estimated in microseconds: a 64-deep K-tile of a 256x256 tile takes 1.7 K-major and 1.48 NT (all CUs busy; the wide NT tiles are
 // 10 % and 5 % better per flop), the transpose and the partials' write and read their bytes at 4.6 and 5 TB/s.
-struct DxPlan { int bm, splits; bool transposed; };
+enum { DX_KMAJOR, DX_TRANSPOSED, DX_RING };
+struct DxPlan { int kind, bm, splits; };
+// a 64-deep K-tile of the 128x128 ring kernel: 0.3 us alone, 0.6 with a block on every CU (L2)
+static double ring_us(long tiles, int cus) { return 0.3 + 0.3 * (double)tiles / cus; }
+static double join_us(int splits, double rows, double cols) { return splits > 1 ? splits * rows * cols * 8 / 5e6 + 6.0 : 0.0; }
 static DxPlan dx_plan(int M, int N, int K) {
     const int cus = device_cu_count(current_device()), kt = N / 64;
-    DxPlan best = {256, 1, false};
+    DxPlan best = {DX_KMAJOR, 256, 1};
     double least = 1e30;
-    auto consider = [&](int bm, int bn, int splits, bool transposed, double per_tile) {
-        const double tiles = (double)ceil_div(M, bm) * ceil_div(K, bn) * splits;
-        const double rounds = (double)(long)((tiles + cus - 1) / cus);
-        const double t = rounds * (ceil_div(kt, splits) * per_tile * bm * bn / 65536.0 + 4.0) + (splits > 1 ? (double)splits * M * K * 8 / 5e6 + 6.0 : 0.0) +
-                         (transposed ? (double)N * K * 4 / 4.6e6 + 4.0 : 0.0);
-        if (t < least) { least = t; best = {bm, splits, transposed}; }
+    auto consider = [&](int kind, int bm, int bn, int splits, double per_tile) {
+        const long tiles = (long)ceil_div(M, bm) * ceil_div(K, bn) * splits;
+        if (kind == DX_RING && tiles > cus) return;
+        const double rounds = (double)((tiles + cus - 1) / cus);
+        if (kind == DX_RING) per_tile = ring_us(tiles, cus);
+        const double t = rounds * (ceil_div(kt, splits) * per_tile + 4.0) + join_us(splits, M, K) + (kind == DX_TRANSPOSED ? (double)N * K * 4 / 4.6e6 + 4.0 : 0.0);
+        if (t < least) { least = t; best = {kind, bm, splits}; }
     };
-    consider(256, 256, 1, false, 1.7);
-    consider(256, 256, 1, true, 1.48);                   // (vitg_gemm picks its own tile: the cheapest of these three)
-    if (K >= 384) consider(256, 384, 1, true, 1.48 / 1.1);
-    if (M >= 384) consider(384, 256, 1, true, 1.48 / 1.05);
-    for (int sp = 2; sp <= 16 && sp * 4 <= kt; ++sp) {
-        consider(256, 256, sp, false, 1.7);
-        consider(256, 256, sp, true, 1.48);
-        if (M > 256) { consider(320, 256, sp, false, 1.67); consider(320, 256, sp, true, 1.45); }
+    consider(DX_KMAJOR, 256, 256, 1, 1.7);
+    consider(DX_TRANSPOSED, 256, 256, 1, 1.48);          // (vitg_gemm picks its own tile: the cheapest of these three)
+    if (K >= 384) consider(DX_TRANSPOSED, 256, 384, 1, 1.48 * 1.5 / 1.1);
+    if (M >= 384) consider(DX_TRANSPOSED, 384, 256, 1, 1.48 * 1.5 / 1.05);
+    for (int sp = 1; sp <= 16 && sp <= kt; ++sp) {
+        consider(DX_RING, 128, 128, sp, 0.0);
+        if (sp < 2 || sp * 4 > kt) continue;
+        consider(DX_KMAJOR, 256, 256, sp, 1.7);
+        consider(DX_TRANSPOSED, 256, 256, sp, 1.48);
+        if (M > 256) { consider(DX_KMAJOR, 320, 256, sp, 1.67 * 1.25); consider(DX_TRANSPOSED, 320, 256, sp, 1.45 * 1.25); }
     }
     return best;
 }
 
 // dW = dGU^T X has a long contraction (the rows) and, for narrow layers, few tiles: the same split, the same estimate
-static int dw_splits(long Mp, int N, int K) {
-    const int cus = device_cu_count(current_device());
-    const long kt = Mp / 64, tiles = (long)ceil_div(N, 256) * ceil_div(K, 256);
-    int best = 1;
+struct DwPlan { bool ring; int splits; };
+static DwPlan dw_plan(long Mp, int N, int K) {
+    const int cus = device_cu_count(current_device()), kt = (int)(Mp / 64);
+    const long wide = (long)ceil_div(N, 256) * ceil_div(K, 256), small = (long)ceil_div(N, 128) * ceil_div(K, 128);
+    DwPlan best = {false, 1};
     double least = 1e30;
-    for (int sp = 1; sp <= 16 && (sp == 1 || sp * 4 <= kt); ++sp) {
-        const double t = (double)((tiles * sp + cus - 1) / cus) * ((double)((kt + sp - 1) / sp) * 1.7 + 4.0) + (sp > 1 ? (double)sp * N * K * 8 / 5e6 + 6.0 : 0.0);
-        if (t < least) { least = t; best = sp; }
+    for (int sp = 1; sp <= 16 && sp <= kt; ++sp) {
+        const double j = join_us(sp, N, K), tw = (double)((wide * sp + cus - 1) / cus) * (ceil_div(kt, sp) * 1.6 + 4.0) + j, tr = ceil_div(kt, sp) * ring_us(small * sp, cus) + 4.0 + j;
+        if ((sp == 1 || sp * 4 <= kt) && tw < least) { least = tw; best = {false, sp}; }
+        if (small * sp <= cus && tr < least) { least = tr; best = {true, sp}; }
     }
     return best;
 }
 
 static size_t pad256(size_t b) { return (b + 255) & ~(size_t)255; }
-struct SwigluWorkspace { size_t dgu, dgut, xt, wt, part, bytes; long Mp; int dx_shares, dw_splits; DxPlan plan; };
+struct SwigluWorkspace { size_t dgu, dgut, xt, wt, part, bytes; long Mp; int dx_shares; DxPlan dx; DwPlan dw; bool pair; };
 static SwigluWorkspace swiglu_workspace(int M, int N, int K, bool dx, bool dw) {
     SwigluWorkspace w = {};
     w.Mp = ((long)M + 63) / 64 * 64;
@@ -349,21 +389,24 @@ static SwigluWorkspace swiglu_workspace(int M, int N, int K, bool dx, bool dw) {
     auto take = [&](size_t bytes) { const size_t a = at; at += pad256(bytes); return a; };
     if (dx) {
         w.dgu = take((size_t)M * N * 2);
-        if (M <= DX_ROWS) { w.dx_shares = dx_shares(N, K); part = (size_t)w.dx_shares * M * K * 4; }
+        if (M <= BWD_ROWS) { w.dx_shares = dx_shares(N, K); part = (size_t)w.dx_shares * M * K * 4; }
         else {
-            w.plan = dx_plan(M, N, K);
-            if (w.plan.transposed) w.wt = take((size_t)K * N * 2);
-            if (w.plan.splits > 1) part = (size_t)w.plan.splits * M * K * 4;
+            w.dx = dx_plan(M, N, K);
+            if (w.dx.kind == DX_TRANSPOSED) w.wt = take((size_t)K * N * 2);
+            if (w.dx.splits > 1) part = (size_t)w.dx.splits * M * K * 4;
         }
     }
     if (dw) {
         w.dgut = take((size_t)N * w.Mp * 2);
-        w.dw_splits = 1;
-        if (M > DW_ROWS) {
+        if (M > BWD_ROWS) {
             w.xt = take((size_t)K * w.Mp * 2);
-            w.dw_splits = dw_splits(w.Mp, N, K);
-            const size_t p = w.dw_splits > 1 ? (size_t)w.dw_splits * N * K * 4 : 0;
-            if (p > part) part = p;                      // (dX's partials are joined before dW's are written)
+            w.dw = dw_plan(w.Mp, N, K);
+            // (one share of the ring kernel needs a partial only where it is added to dW or shares a launch with dX)
+            const size_t p = w.dw.splits > 1 || w.dw.ring ? (size_t)w.dw.splits * N * K * 4 : 0;
+            // two ring products share one launch and one join: fewer launches, and the smaller one fills the CUs that the other leaves
+            w.pair = dx && w.dw.ring && w.dx.kind == DX_RING;
+            if (w.pair) part = (size_t)w.dx.splits * M * K * 4 + p;
+            else if (p > part) part = p;                 // (dX's partials are joined before dW's are written)
         }
     }
     w.part = take(part);
@@ -398,10 +441,11 @@ extern "C" int vitg_swiglu(const void* X, int ldx, const void* W, int ldw, int M
     GemmArgs g = {};
     g.A = X; g.lda = ldx; g.W = W; g.ldw = ldw; g.M = M; g.N = N; g.K = K;
     g.out = out; g.ldo = ldo; g.gu = gu; g.ldgu = ldgu; g.split_k = 1;
-    // the 128x128 tile while its tiles fit the chip once (K = 1024, N = 4096, 1 024 rows: 17.6 us against 23.5 on 256x256) and up to 128 rows (a 256-row tile
-    // would be half empty: 73 against 100 us at 3584 x 37888); beyond that the 256-row tiles
+    // at most one 128x128 tile per CU: the ring kernel.  Up to 128 rows the 128x128 tile at two blocks per CU (a 256-row tile would be half empty: 73 against
+    // 100 us at 3584 x 37888); beyond that the 256-row tiles
     int rc;
-    if (M <= 128 || (long)ceil_div(M, 128) * ceil_div(N, 128) <= device_cu_count(current_device())) rc = launch_gemm128_swiglu(g, dtype, s);
+    if ((long)ceil_div(M, 128) * ceil_div(N, 128) <= device_cu_count(current_device())) rc = launch_gemm_ring(g, dtype, MODE_SWIGLU, false, s);
+    else if (M <= 128) rc = launch_gemm128_swiglu(g, dtype, s);
     else if (gu) rc = launch_gemm_mi16_swiglu_save(g, dtype, s);
     else if (M < 256) rc = launch_gemm_mi16(g, dtype, MODE_SWIGLU, 6, s);
     else return vitg_gemm(X, ldx, W, ldw, M, N, K, dtype, VITG_GEMM_SWIGLU, nullptr, VITG_ACT_NONE, out, ldo, nullptr, 0, 0, stream);
@@ -436,52 +480,70 @@ extern "C" int vitg_swiglu_backward(const void* dout, int lddo, const void* gu, 
     const SwigluWorkspace ws = swiglu_workspace(M, N, K, dX != nullptr, dW != nullptr);
     if (!workspace || workspace_bytes < (long)ws.bytes || !aligned_to(workspace, 16)) return VITG_ERR_ARG;
     char* const base = (char*)workspace;
-    void *dgu = dX ? base + ws.dgu : nullptr, *dgut = dW ? base + ws.dgut : nullptr, *xt = base + ws.xt;
-    const unsigned mt = (unsigned)(ws.Mp / 64);
+    void *const dgu = dX ? base + ws.dgu : nullptr, *const dgut = dW ? base + ws.dgut : nullptr, *const xt = base + ws.xt;
     float* const part = (float*)(base + ws.part);
     auto run = [&](auto t) -> int {
         typedef decltype(t) T;
-        hipLaunchKernelGGL(swiglu_grad_kernel<T>, dim3(mt, N / 64), dim3(256), 0, s, (const T*)dout, (long)lddo, (const T*)gu, (long)ldgu, (long)M, ws.Mp, (T*)dgu, (long)N, (T*)dgut);
-        if (dX && M <= DX_ROWS) {
-            auto go = [&](auto kernel) {
-                hipLaunchKernelGGL(kernel, dim3(ceil_div(K, 128), ws.dx_shares), dim3(256), 0, s, (const T*)dgu, (long)N, (const T*)W, (long)ldw, M, N, K, ws.dx_shares, part);
-            };
-            if (M <= 16) go(swiglu_dx_rows_kernel<T, 1>); else go(swiglu_dx_rows_kernel<T, 2>);
-            join_shares<T>(part, M, K, ws.dx_shares, dX, lddx, 0, s);
-        } else if (dX) {
-            GemmArgs g = {};
-            g.A = dgu; g.lda = N; g.W = W; g.ldw = ldw; g.M = M; g.N = K; g.K = N;
-            g.split_k = ws.plan.splits;
-            if (ws.plan.splits > 1) { g.out = part; g.ldo = K; g.split_stride = (long)M * K; }
-            else { g.out = dX; g.ldo = lddx; }
-            if (ws.plan.transposed) {
-                hipLaunchKernelGGL(transpose16_kernel<T>, dim3(N / 64, K / 64), dim3(256), 0, s, (const T*)W, (long)ldw, (long)N, K, (T*)(base + ws.wt), (long)N, (long)N);
-                g.W = base + ws.wt; g.ldw = N;
-            }
-            int rc;
-            if (!ws.plan.transposed) rc = launch_gemm_mi16_kmajor(g, dtype, ws.plan.bm, s);
-            else if (ws.plan.splits > 1) rc = launch_gemm_mi16(g, dtype, MODE_F32, ws.plan.bm == 320 ? 12 : 6, s);
-            else rc = vitg_gemm(dgu, N, g.W, N, M, K, N, dtype, VITG_GEMM_STORE16, nullptr, VITG_ACT_NONE, dX, lddx, nullptr, 0, 0, stream);
-            if (rc) return VITG_ERR_LAUNCH;
-            if (ws.plan.splits > 1) join_shares<T>(part, M, K, ws.plan.splits, dX, lddx, 0, s);
+        const bool few = M <= BWD_ROWS, pair = !few && dX && dW && ws.pair;
+        {
+            const long mt = ws.Mp / 64;
+            SwigluPrep<T> a = {(const T*)dout, (long)lddo, (const T*)gu, (long)ldgu, (long)M, ws.Mp, (T*)dgu, (long)N, (T*)dgut,
+                               (const T*)X, (long)ldx, (T*)xt, (const T*)W, (long)ldw, (T*)(base + ws.wt), N, K, mt * (N / 64), 0};
+            a.x_end = a.grad + (dW && !few ? mt * (K / 64) : 0);
+            const long blocks = a.x_end + (dX && !few && ws.dx.kind == DX_TRANSPOSED ? (long)(N / 64) * (K / 64) : 0);
+            hipLaunchKernelGGL(swiglu_prep_kernel<T>, dim3((unsigned)blocks), dim3(256), 0, s, a);
         }
-        if (dW && M <= DW_ROWS) {
+        const JoinArgs join_dx = {part, M, K, few ? ws.dx_shares : ws.dx.splits, dX, lddx, 0};
+        if (few) {
+            const int columns = ceil_div(K, 128), nx = dX ? columns * ws.dx_shares : 0, nw = dW ? columns * ceil_div(N, 4 * DW_WAVE) : 0;
             auto go = [&](auto tw) {
                 typedef decltype(tw) TW;
-                hipLaunchKernelGGL((swiglu_dw_rows_kernel<T, TW>), dim3(ceil_div(K, 128), ceil_div(N, 256)), dim3(256), 0, s, (const T*)dgut, ws.Mp, (const T*)X, (long)ldx, M, N, K, (TW*)dW, (long)lddw, accumulate);
+                auto launch = [&](auto kernel) {
+                    hipLaunchKernelGGL(kernel, dim3(nx + nw), dim3(256), 0, s, (const T*)dgu, (const T*)W, (long)ldw, M, N, K, ws.dx_shares, part, nx, (const T*)dgut, ws.Mp, (const T*)X, (long)ldx, (TW*)dW, (long)lddw, accumulate);
+                };
+                if (M <= 16) launch(swiglu_rows_backward_kernel<T, TW, 1>); else launch(swiglu_rows_backward_kernel<T, TW, 2>);
             };
-            if (dw_dtype == DT_F32) go(float{}); else go(t);
-        } else if (dW) {
-            void* const xt = base + ws.xt;
-            const int Mp = (int)ws.Mp;
-            hipLaunchKernelGGL(transpose16_kernel<T>, dim3(mt, K / 64), dim3(256), 0, s, (const T*)X, (long)ldx, (long)M, K, (T*)xt, ws.Mp, ws.Mp);
-            if (ws.dw_splits > 1) {
-                GemmArgs g = {};
-                g.A = dgut; g.lda = Mp; g.W = xt; g.ldw = Mp; g.M = N; g.N = K; g.K = Mp;
-                g.split_k = ws.dw_splits; g.out = part; g.ldo = K; g.split_stride = (long)N * K;
-                if (launch_gemm_mi16(g, dtype, MODE_F32, 6, s) != 0) return VITG_ERR_LAUNCH;
-                if (dw_dtype == DT_F32) join_shares<float>(part, N, K, ws.dw_splits, dW, lddw, accumulate, s);
-                else join_shares<T>(part, N, K, ws.dw_splits, dW, lddw, accumulate, s);
+            if (dW && dw_dtype == DT_F32) go(float{}); else go(t);
+            if (dX) join_shares<T>(join_dx, s);
+            return launched();
+        }
+        GemmArgs gx = {}, gw = {};
+        const int Mp = (int)ws.Mp;
+        if (dX) {
+            const DxPlan p = ws.dx;
+            gx.A = dgu; gx.lda = N; gx.W = W; gx.ldw = ldw; gx.M = M; gx.N = K; gx.K = N; gx.split_k = p.splits;
+            if (p.splits > 1 || pair) { gx.out = part; gx.ldo = K; gx.split_stride = (long)M * K; }
+            else { gx.out = dX; gx.ldo = lddx; }
+            if (p.kind == DX_TRANSPOSED) { gx.W = base + ws.wt; gx.ldw = N; }
+        }
+        if (dW) {
+            gw.A = dgut; gw.lda = Mp; gw.W = xt; gw.ldw = Mp; gw.M = N; gw.N = K; gw.K = Mp; gw.split_k = ws.dw.splits;
+            gw.out = pair ? part + (size_t)ws.dx.splits * M * K : part; gw.ldo = K; gw.split_stride = (long)N * K;
+        }
+        const JoinArgs join_dw = {(const float*)gw.out, N, K, ws.dw.splits, dW, lddw, accumulate};
+        if (pair) {
+            if (launch_gemm_ring_pair(gx, gw, dtype, s) != 0) return VITG_ERR_LAUNCH;
+            if (dw_dtype == DT_F32) join_shares<T, float>(join_dx, s, join_dw); else join_shares<T, T>(join_dx, s, join_dw);
+            return launched();
+        }
+        if (dX) {
+            const DxPlan p = ws.dx;
+            int rc;
+            if (p.kind == DX_RING) rc = launch_gemm_ring(gx, dtype, p.splits > 1 ? MODE_F32 : MODE_STORE16, true, s);
+            else if (p.kind == DX_KMAJOR) rc = launch_gemm_mi16_kmajor(gx, dtype, p.bm, s);
+            else if (p.splits > 1) rc = launch_gemm_mi16(gx, dtype, MODE_F32, p.bm == 320 ? 12 : 6, s);
+            else rc = vitg_gemm(dgu, N, gx.W, N, M, K, N, dtype, VITG_GEMM_STORE16, nullptr, VITG_ACT_NONE, dX, lddx, nullptr, 0, 0, stream);
+            if (rc) return VITG_ERR_LAUNCH;
+            if (p.splits > 1) join_shares<T>(join_dx, s);
+        }
+        if (dW) {
+            const DwPlan p = ws.dw;
+            if (p.ring && p.splits == 1 && !accumulate && dw_dtype != DT_F32) {
+                gw.out = dW; gw.ldo = lddw;
+                if (launch_gemm_ring(gw, dtype, MODE_STORE16, false, s) != 0) return VITG_ERR_LAUNCH;
+            } else if (p.ring || p.splits > 1) {
+                if ((p.ring ? launch_gemm_ring(gw, dtype, MODE_F32, false, s) : launch_gemm_mi16(gw, dtype, MODE_F32, 6, s)) != 0) return VITG_ERR_LAUNCH;
+                if (dw_dtype == DT_F32) join_shares<float>(join_dw, s); else join_shares<T>(join_dw, s);
             } else {
                 const int rc = dw_dtype == DT_F32
                     ? vitg_gemm(dgut, Mp, xt, Mp, N, K, Mp, dtype, VITG_GEMM_F32, nullptr, VITG_ACT_NONE, dW, lddw, accumulate ? (const float*)dW : nullptr, lddw, 0, stream)

@@ -2,7 +2,9 @@
 typed views of HBM; every call goes to libvideoitg_hip.so on torch's current stream.  No torch math here."""
 from __future__ import annotations
 
+import array
 import ctypes as C
+import functools
 from typing import Optional
 
 import torch
@@ -631,13 +633,21 @@ def _same_device(*tensors: Optional[torch.Tensor]) -> int:
     return idx
 
 
+_entries = {}
+
+
 def _call_on(idx: int, name: str, *args) -> None:
     """the entry point on device idx and its current stream (the last argument)"""
-    if torch.cuda.current_device() == idx:
-        _lib.check(getattr(_lib.load(), name)(*args, _raw_stream(idx)), name)
+    fn = _entries.get(name)
+    if fn is None:
+        fn = _entries[name] = getattr(_lib.load(), name)
+    if torch._C._cuda_getDevice() == idx:
+        rc = fn(*args, _raw_stream(idx))
     else:
         with torch.cuda.device(idx):
-            _lib.check(getattr(_lib.load(), name)(*args, _raw_stream(idx)), name)
+            rc = fn(*args, _raw_stream(idx))
+    if rc:
+        _lib.check(rc, name)
 
 
 def _matrix(t: torch.Tensor, what: str, rows: int, cols: int, dtypes):
@@ -713,6 +723,7 @@ def embed_lookup(ids: torch.Tensor, table: torch.Tensor, out: torch.Tensor, *, s
     return out
 
 
+@functools.lru_cache(maxsize=1024)
 def embed_backward_plan(n: int, d: int) -> int:
     """workspace bytes of embed_backward for n tokens of width d"""
     b = C.c_long(0)
@@ -753,6 +764,7 @@ def swiglu(x: torch.Tensor, w: torch.Tensor, out: torch.Tensor, *, gu: Optional[
     return out
 
 
+@functools.lru_cache(maxsize=1024)
 def swiglu_backward_plan(m: int, n: int, k: int, want_dx: bool = True, want_dw: bool = True) -> int:
     """workspace bytes of swiglu_backward for x [m, k] and w [n, k]"""
     b = C.c_long(0)
@@ -883,11 +895,12 @@ def clip_grad_norm(grads, max_norm: Optional[float], *, outs=None, scale: float 
     if norm is None:
         norm = torch.empty(1, dtype=torch.float32, device=idx)
     pn, en = _vector(norm, "norm", 1, torch.float32)
-    longs, pointers = C.c_long * n, C.c_void_p * n
-    numel, codes, need = longs(*numel), (C.c_int * n)(*codes), C.c_long(0)
-    _lib.call("vitg_clip_grad_plan", n, numel, codes, C.byref(need))
+    sizes, kinds, src = array.array("l", numel), array.array("i", codes), array.array("L", pin)
+    dst = None if pout is None else src if pout is pin else array.array("L", pout)
+    ps, pk, need = sizes.buffer_info()[0], kinds.buffer_info()[0], C.c_long(0)
+    _lib.call("vitg_clip_grad_plan", n, ps, pk, C.byref(need))
     ws, pw, nw = _workspace(workspace, need.value, idx)
     _distinct([("norm", pn, en), ("workspace", pw, pw + nw)])
-    _call_on(idx, "vitg_clip_grad", n, pointers(*pin), None if pout is None else pointers(*pout), numel, codes, scale, 0.0 if max_norm is None else max_norm,
+    _call_on(idx, "vitg_clip_grad", n, src.buffer_info()[0], None if dst is None else dst.buffer_info()[0], ps, pk, scale, 0.0 if max_norm is None else max_norm,
              pn, pw, nw)
     return norm
