@@ -270,7 +270,7 @@ template <typename TA, typename TB = TA> static void join_shares(const JoinArgs&
 // dW (+)= dGU^T X for M <= 32 rows: a wave owns 32 rows x 128 columns of dW.  A = X transposed in registers (as above), B = dGU^T rows from the transposed copy.
 // Bound by the write of dW.
 constexpr int DW_WAVE = 32;
-template <typename T, typename TW>
+template <typename T, typename TW, bool AROUND>
 __device__ __forceinline__ void dw_rows_block(int column, int rows, const T* __restrict__ dgut, long Mp, const T* __restrict__ X, long ldx, int M, int N, int K,
                                               TW* __restrict__ dW, long lddw, int accumulate) {
     typedef typename T16<T>::vec8 vec8;
@@ -306,18 +306,18 @@ __device__ __forceinline__ void dw_rows_block(int column, int rows, const T* __r
             if (accumulate) load_vec<TW, 8>(o, v);
 #pragma unroll
             for (int j = 0; j < 8; ++j) v[j] = accumulate ? v[j] + acc[i][j][r] : acc[i][j][r];
-            store_vec<TW, 8>(o, v);
+            store_stream<TW, 8, AROUND>(o, v);
         }
 }
 
 // both in one launch - dX reads W while dW is written: blocks [0, dx_blocks) dX (columns fastest), the others dW
-template <typename T, typename TW, int MT>
+template <typename T, typename TW, int MT, bool AROUND>
 __global__ __launch_bounds__(256) void swiglu_rows_backward_kernel(const T* __restrict__ dgu, const T* __restrict__ W, long ldw, int M, int N, int K, int shares,
                                                                    float* __restrict__ part, int dx_blocks, const T* __restrict__ dgut, long Mp,
                                                                    const T* __restrict__ X, long ldx, TW* __restrict__ dW, long lddw, int accumulate) {
     const int columns = (K + 127) / 128, id = blockIdx.x;
     if (id < dx_blocks) dx_rows_block<T, MT>(id % columns, id / columns, dgu, N, W, ldw, M, N, K, shares, part);
-    else dw_rows_block<T, TW>((id - dx_blocks) % columns, (id - dx_blocks) / columns, dgut, Mp, X, ldx, M, N, K, dW, lddw, accumulate);
+    else dw_rows_block<T, TW, AROUND>((id - dx_blocks) % columns, (id - dx_blocks) / columns, dgut, Mp, X, ldx, M, N, K, dW, lddw, accumulate);
 }
 
 // rows that the three kernels take, against the GEMM forms at 3584 x 37888 (us): forward 61 - 74 at 1 - 16 rows, the 128-row tile 69 - 75 at 17 - 128;
@@ -333,12 +333,17 @@ static int dx_shares(int N, int K) {
 // dX = dGU W for more rows: the GEMM with the K-major weight operand (gemm_mi16.hip), or a tile transpose of W in front of the NT GEMM, whose main loop is faster
 // (12 860 rows: 2.43 + 0.12 ms against 2.78; 1 607 rows: 0.41 + 0.12 against 0.43).  Either may split its contraction (N) into fp32 partials where one round
 // of tiles leaves CUs idle.  Estimated in microseconds: a 64-deep K-tile of a 256x256 tile takes 1.7 K-major and 1.48 NT (all CUs busy; the wide NT tiles are
-// 10 % and 5 % better per flop), the transpose and the partials' write and read their bytes at 4.6 and 5 TB/s.
+// 10 % and 5 % better per flop), the transpose moves its bytes at 4.6 TB/s.  Small problems run on the ring kernel (gemm_ring.hip).  Against every alternative
+// forced in turn on 40 shapes (448 .. 3584 x 1024 .. 37888, 40 .. 4 096 rows) the estimate's choice was within 10 % of the best.
 enum { DX_KMAJOR, DX_TRANSPOSED, DX_RING };
 struct DxPlan { int kind, bm, splits; };
-// a 64-deep K-tile of the 128x128 ring kernel: 0.3 us alone, 0.6 with a block on every CU (L2)
-static double ring_us(long tiles, int cus) { return 0.3 + 0.3 * (double)tiles / cus; }
-static double join_us(int splits, double rows, double cols) { return splits > 1 ? splits * rows * cols * 8 / 5e6 + 6.0 : 0.0; }
+// a 64-deep K-tile of the 128x128 ring kernel: 0.35 us alone, 0.7 with a block on every CU (L2)
+static double ring_us(long tiles, int cus) { return 0.35 + 0.35 * (double)tiles / cus; }
+// the partials' write and read, and a launch; up to ~120 MB they stay in the last-level cache
+static double join_us(int splits, double rows, double cols) {
+    const double bytes = splits * rows * cols * 8;
+    return splits > 1 ? 3.0 + bytes / (bytes < 1.2e8 ? 10e6 : 5e6) : 0.0;
+}
 static DxPlan dx_plan(int M, int N, int K) {
     const int cus = device_cu_count(current_device()), kt = N / 64;
     DxPlan best = {DX_KMAJOR, 256, 1};
@@ -441,11 +446,14 @@ extern "C" int vitg_swiglu(const void* X, int ldx, const void* W, int ldw, int M
     GemmArgs g = {};
     g.A = X; g.lda = ldx; g.W = W; g.ldw = ldw; g.M = M; g.N = N; g.K = K;
     g.out = out; g.ldo = ldo; g.gu = gu; g.ldgu = ldgu; g.split_k = 1;
-    // at most one 128x128 tile per CU: the ring kernel.  Up to 128 rows the 128x128 tile at two blocks per CU (a 256-row tile would be half empty: 73 against
-    // 100 us at 3584 x 37888); beyond that the 256-row tiles
+    // at most one 128x128 tile per CU: the ring kernel (K = 1024, N = 4096, 512 rows: 12 us against 16 on the 128x128 tile and 23 on 256x256).  Up to 128 rows,
+    // and with pre-activations up to two tiles per CU, the 128x128 tile at two blocks per CU (3584 x 37888, 128 rows: 73 against 100 us on a half-empty
+    // 256-row tile; 2048 x 16384, 512 rows: 43 against 47); beyond that the 256-row tiles (1 024 rows: 57 against 80)
+    const long tiles = (long)ceil_div(M, 128) * ceil_div(N, 128);
+    const int cus = device_cu_count(current_device());
     int rc;
-    if ((long)ceil_div(M, 128) * ceil_div(N, 128) <= device_cu_count(current_device())) rc = launch_gemm_ring(g, dtype, MODE_SWIGLU, false, s);
-    else if (M <= 128) rc = launch_gemm128_swiglu(g, dtype, s);
+    if (tiles <= cus) rc = launch_gemm_ring(g, dtype, MODE_SWIGLU, false, s);
+    else if (M <= 128 || (gu && tiles <= 2 * cus)) rc = launch_gemm128_swiglu(g, dtype, s);
     else if (gu) rc = launch_gemm_mi16_swiglu_save(g, dtype, s);
     else if (M < 256) rc = launch_gemm_mi16(g, dtype, MODE_SWIGLU, 6, s);
     else return vitg_gemm(X, ldx, W, ldw, M, N, K, dtype, VITG_GEMM_SWIGLU, nullptr, VITG_ACT_NONE, out, ldo, nullptr, 0, 0, stream);
@@ -501,7 +509,10 @@ extern "C" int vitg_swiglu_backward(const void* dout, int lddo, const void* gu, 
                 auto launch = [&](auto kernel) {
                     hipLaunchKernelGGL(kernel, dim3(nx + nw), dim3(256), 0, s, (const T*)dgu, (const T*)W, (long)ldw, M, N, K, ws.dx_shares, part, nx, (const T*)dgut, ws.Mp, (const T*)X, (long)ldx, (TW*)dW, (long)lddw, accumulate);
                 };
-                if (M <= 16) launch(swiglu_rows_backward_kernel<T, TW, 1>); else launch(swiglu_rows_backward_kernel<T, TW, 2>);
+                with_flag((long)N * K * (long)sizeof(TW) > STREAM_BYTES, [&](auto around) {
+                    constexpr bool AROUND = decltype(around)::value;
+                    if (M <= 16) launch(swiglu_rows_backward_kernel<T, TW, 1, AROUND>); else launch(swiglu_rows_backward_kernel<T, TW, 2, AROUND>);
+                });
             };
             if (dW && dw_dtype == DT_F32) go(float{}); else go(t);
             if (dX) join_shares<T>(join_dx, s);

@@ -89,7 +89,7 @@ __global__ __launch_bounds__(CLIP_THREADS) void grad_sumsq_kernel(const ClipArgs
     if (threadIdx.x == 0) sums[blockIdx.x] = s;
 }
 
-template <typename T>
+template <bool AROUND, typename T>
 __device__ __forceinline__ void clip_scale_piece(const T* p, T* q, long count, float factor, int tid) {
     constexpr int V = 16 / sizeof(T);
     long done = 0;
@@ -104,7 +104,7 @@ __device__ __forceinline__ void clip_scale_piece(const T* p, T* q, long count, f
             for (int u = 0; u < 4; ++u) {
 #pragma unroll
                 for (int e = 0; e < V; ++e) v[u][e] *= factor;
-                store_vec<T, V>(q + i + u * CLIP_THREADS * V, v[u]);
+                store_stream<T, V, AROUND>(q + i + u * CLIP_THREADS * V, v[u]);
             }
         }
         for (; i < done; i += CLIP_THREADS * V) {
@@ -125,6 +125,7 @@ __device__ __forceinline__ double clip_norm(const double* __restrict__ sums, int
     return sqrt(block_sum_f64(s, red)) * fabs((double)scale);
 }
 
+template <bool AROUND>
 __global__ __launch_bounds__(CLIP_THREADS) void grad_scale_kernel(const ClipArgs a, const double* __restrict__ sums, int nsums, float scale, float max_norm,
                                                                   float* __restrict__ norm_out) {
     __shared__ double red[4];
@@ -134,14 +135,15 @@ __global__ __launch_bounds__(CLIP_THREADS) void grad_scale_kernel(const ClipArgs
     const double clip = max_norm == INFINITY ? 1.0 : (double)max_norm / (norm + 1e-6);
     const float factor = (float)((double)scale * (clip < 1.0 ? clip : clip != clip ? clip : 1.0));
     const int pieces = a.count ? a.piece0[a.count] : 0;
-    for (int p = blockIdx.x; p < pieces; p += gridDim.x) {
+    // from the end: what pass 1 read last is still in the last-level cache
+    for (int p = pieces - 1 - (int)blockIdx.x; p >= 0; p -= gridDim.x) {
         const int t = clip_find(a, p);
         if (factor == 1.0f && a.in[t] == a.out[t]) continue;                    // in place and nothing to scale
         const int esize = a.dtype[t] == DT_F32 ? 4 : 2;
         const long per = CLIP_PIECE / esize, at = (long)(p - a.piece0[t]) * per, count = min(per, a.numel[t] - at);
-        if (a.dtype[t] == DT_BF16) clip_scale_piece((const bf16_t*)a.in[t] + at, (bf16_t*)a.out[t] + at, count, factor, threadIdx.x);
-        else if (a.dtype[t] == DT_F16) clip_scale_piece((const f16_t*)a.in[t] + at, (f16_t*)a.out[t] + at, count, factor, threadIdx.x);
-        else clip_scale_piece((const float*)a.in[t] + at, (float*)a.out[t] + at, count, factor, threadIdx.x);
+        if (a.dtype[t] == DT_BF16) clip_scale_piece<AROUND>((const bf16_t*)a.in[t] + at, (bf16_t*)a.out[t] + at, count, factor, threadIdx.x);
+        else if (a.dtype[t] == DT_F16) clip_scale_piece<AROUND>((const f16_t*)a.in[t] + at, (f16_t*)a.out[t] + at, count, factor, threadIdx.x);
+        else clip_scale_piece<AROUND>((const float*)a.in[t] + at, (float*)a.out[t] + at, count, factor, threadIdx.x);
     }
 }
 
@@ -277,11 +279,15 @@ extern "C" int vitg_clip_grad(int count, const void* const* grads, void* const* 
         hipLaunchKernelGGL(grad_norm_kernel, dim3(1), dim3(CLIP_THREADS), 0, s, sums, nsums, scale, norm);
         return launched();
     }
+    long bytes = 0;
+    for (int i = 0; i < count; ++i) bytes += numel[i] * dtype_size(dtype[i]);
     bool first = true;
     for (int at = 0; at < count; first = false) {
         at = clip_fill(a, at, count, grads, outs, numel, dtype);
         if (!a.count) break;
-        hipLaunchKernelGGL(grad_scale_kernel, dim3(clip_blocks(a.piece0[a.count])), dim3(CLIP_THREADS), 0, s, a, sums, nsums, scale, max_norm, first ? norm : (float*)nullptr);
+        with_flag(bytes > STREAM_BYTES, [&](auto around) {
+            hipLaunchKernelGGL(grad_scale_kernel<decltype(around)::value>, dim3(clip_blocks(a.piece0[a.count])), dim3(CLIP_THREADS), 0, s, a, sums, nsums, scale, max_norm, first ? norm : (float*)nullptr);
+        });
     }
     return launched();
 }

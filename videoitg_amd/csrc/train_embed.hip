@@ -237,71 +237,70 @@ __global__ __launch_bounds__(256) void embed_grad_kernel(const unsigned* __restr
     store_vec<float, V>(partial + ((size_t)blockIdx.x * 2 + (began ? 1 : 0)) * ((size_t)cv * V) + (size_t)c * V, acc);
 }
 
-// runs across chunks: the block of the chunk in which a run begins adds its partials in chunk order.  16 waves: four column groups of 256 columns, four
-// consecutive parts of the list each; the parts' sums join through LDS in order
-constexpr int JOIN_PARTS = 4, JOIN_COLS = 1024;
+// runs across chunks: the partials of a run are added in chunk order by the wave (short lists) or the block (long ones) of the chunk in which it begins.  A block
+// looks at 16 chunks, one per wave, and JOIN_COLS columns; a long list is cut into eight consecutive parts whose sums join through LDS in order.
+constexpr int JOIN_PARTS = 8, JOIN_COLS = 512, JOIN_SHORT = 8;
 template <typename TT>
 __global__ __launch_bounds__(1024) void embed_join_kernel(const unsigned* __restrict__ key, long n, unsigned vocab, int chunk, int D, float scale,
                                                           TT* __restrict__ table, long ldt, int accumulate, const float* __restrict__ partial) {
     constexpr int V = 4;
     __shared__ float part[JOIN_PARTS][JOIN_COLS];
-    __shared__ unsigned begins[16];
+    __shared__ int items_of[16];
     const long chunks = (n + chunk - 1) / chunk;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, p = wave >> 2;
-    if (lane == 0) {                                     // wave w looks at chunk 16 blockIdx.x + w: does a run that goes on behind it begin there
-        const long b = blockIdx.x * 16l + wave;
-        unsigned is = 0;
-        if (b + 1 < chunks) {
-            const unsigned run = key[(b + 1) * chunk - 1];
-            is = run < vocab && key[(b + 1) * chunk] == run && !(b > 0 && key[b * chunk - 1] == run);
-        }
-        begins[wave] = is;
-    }
-    __syncthreads();
-    for (int w16 = 0; w16 < 16; ++w16) {
-    if (!begins[w16]) continue;                          // (the same for every thread of the block)
-    const long b = blockIdx.x * 16l + w16;
-    const unsigned run = key[(b + 1) * chunk - 1];
-    long last = b + 1;                                   // last chunk that holds a part of the run
-    for (;;) {
-        const long j = last + 1 + lane;
-        const unsigned long long in = __ballot(j < chunks && key[min(j, chunks - 1) * chunk] == run);
-        const int more = in == ~0ull ? 64 : __ffsll((unsigned long long)~in) - 1;
-        last += more;
-        if (more < 64) break;
-    }
-    const int at = (wave & 3) * 256 + lane * V, c = blockIdx.y * JOIN_COLS + at;
-    const long items = last - b + 1, per = (items + JOIN_PARTS - 1) / JOIN_PARTS, i0 = p * per, i1 = min(i0 + per, items);
-    float acc[V] = {0.f, 0.f, 0.f, 0.f};
-    if (c < D) {
-        // item i: the part that chunk b + i holds (slot 1 of the first, slot 0 of the others)
-        auto item = [&](long i) { return partial + ((size_t)(b + i) * 2 + (i == 0 ? 1 : 0)) * (size_t)D + c; };
-        long i = i0;
-        for (; i + 8 <= i1; i += 8) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, p = wave >> 1, c0 = blockIdx.y * JOIN_COLS;
+    // item i of the run that begins in chunk b: the part that chunk b + i holds (slot 1 of the first, slot 0 of the others)
+    auto item = [&](long b, long i, int c) { return partial + ((size_t)(b + i) * 2 + (i == 0 ? 1 : 0)) * (size_t)D + c; };
+    auto add = [&](long b, long i0, long i1, int c, float (&acc)[V]) {
+        for (long i = i0; i < i1; i += 8) {              // eight in flight; past the end the last one again, left out of the sum
             float v[8][V];
 #pragma unroll
-            for (int g = 0; g < 8; ++g) load_vec<float, V>(item(i + g), v[g]);
+            for (int g = 0; g < 8; ++g) load_vec<float, V>(item(b, min(i + g, i1 - 1), c), v[g]);
 #pragma unroll
             for (int g = 0; g < 8; ++g)
+                if (i + g < i1)
 #pragma unroll
-                for (int k = 0; k < V; ++k) acc[k] += v[g][k];
+                    for (int k = 0; k < V; ++k) acc[k] += v[g][k];
         }
-        for (; i < i1; ++i) {
-            float v[V];
-            load_vec<float, V>(item(i), v);
-#pragma unroll
-            for (int k = 0; k < V; ++k) acc[k] += v[k];
+    };
+    const long mine = blockIdx.x * 16l + wave;
+    int items = 0;                                       // parts of the run that begins in this wave's chunk and goes on behind it
+    if (mine + 1 < chunks) {
+        const unsigned run = key[(mine + 1) * chunk - 1];
+        if (run < vocab && key[(mine + 1) * chunk] == run && !(mine > 0 && key[mine * chunk - 1] == run)) {
+            items = 2;
+            for (;;) {                                   // 64 chunks at a time: does the run reach into them
+                const long j = mine + items + lane;
+                const unsigned long long in = __ballot(j < chunks && key[min(j, chunks - 1) * chunk] == run);
+                const int more = in == ~0ull ? 64 : __ffsll((unsigned long long)~in) - 1;
+                items += more;
+                if (more < 64) break;
+            }
+            if (items <= JOIN_SHORT)
+                for (int c = c0 + lane * V; c < min(c0 + JOIN_COLS, D); c += 64 * V) {
+                    float acc[V] = {0.f, 0.f, 0.f, 0.f};
+                    add(mine, 0, items, c, acc);
+                    finish_row<TT, V>(table + (long)run * ldt + c, accumulate, scale, acc);
+                }
         }
     }
-    store_vec<float, V>(&part[p][at], acc);
+    if (lane == 0) items_of[wave] = items;
     __syncthreads();
-    if (p == 0 && c < D) {
-        for (int w = 1; w < JOIN_PARTS; ++w)
+    for (int w = 0; w < 16; ++w) {
+        const int count = items_of[w];                   // (the same for every thread of the block)
+        if (count <= JOIN_SHORT) continue;
+        const long b = blockIdx.x * 16l + w;
+        const int at = (wave & 1) * 256 + lane * V, c = c0 + at, per = (count + JOIN_PARTS - 1) / JOIN_PARTS;
+        float acc[V] = {0.f, 0.f, 0.f, 0.f};
+        if (c < D) add(b, p * per, min((p + 1) * per, count), c, acc);
+        store_vec<float, V>(&part[p][at], acc);
+        __syncthreads();
+        if (p == 0 && c < D) {
+            for (int q = 1; q < JOIN_PARTS; ++q)
 #pragma unroll
-            for (int k = 0; k < V; ++k) acc[k] += part[w][at + k];
-        finish_row<TT, V>(table + (long)run * ldt + c, accumulate, scale, acc);
-    }
-    __syncthreads();
+                for (int k = 0; k < V; ++k) acc[k] += part[q][at + k];
+            finish_row<TT, V>(table + (long)key[(b + 1) * chunk - 1] * ldt + c, accumulate, scale, acc);
+        }
+        __syncthreads();
     }
 }
 

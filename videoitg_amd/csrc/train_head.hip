@@ -7,13 +7,14 @@
 //
 // The backward of the mean needs no second look at h: the forward keeps the frame means (frames x D fp32, 1 / tokens of h), so a step reads h once and
 // writes dh once - HBM-bound on both sides.
+#include <type_traits>
 #include "train_common.h"
 
 namespace vitg {
 
 // One block per frame when there are enough frames to fill the chip; otherwise the columns of a frame are spread over gridDim.y blocks (SCORE = false) and
 // pool_dot_kernel takes the scores from the means.
-template <typename T, int V, bool SCORE>
+template <typename T, int V, bool SCORE, bool AROUND>
 __global__ __launch_bounds__(1024) void pool_score_save_kernel(const T* __restrict__ h, long ldh, int tokens, int cv, const float* __restrict__ w,
                                                                const float* __restrict__ b, float* __restrict__ logits, float* __restrict__ pooled, long ldp) {
     const long t = blockIdx.x;
@@ -27,7 +28,7 @@ __global__ __launch_bounds__(1024) void pool_score_save_kernel(const T* __restri
 #pragma unroll 5
         for (int j = 0; j < tokens; ++j) {
             float v[V];
-            load_vec<T, V>(p + j * ldh, v);
+            load_stream<T, V, AROUND>(p + j * ldh, v);
 #pragma unroll
             for (int e = 0; e < V; ++e) s[e] += v[e];
         }
@@ -181,9 +182,13 @@ extern "C" int vitg_pool_score_save(const void* h, int h_dtype, long ldh, int fr
     with_dtype(h_dtype, [&](auto ti) {
         typedef decltype(ti) T;
         auto run = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(threads), 0, s, (const T*)h, ldh, tokens_per_frame, cv, w, b, logits, pooled, ldp); };
-        if (few) { if (wide) run(pool_score_save_kernel<T, 8, false>); else run(pool_score_save_kernel<T, 4, false>); }
-        else if (wide) run(pool_score_save_kernel<T, 8, true>);
-        else run(pool_score_save_kernel<T, 4, true>);
+        auto pick = [&](auto around) {
+            constexpr bool AROUND = decltype(around)::value;
+            if (few) { if (wide) run(pool_score_save_kernel<T, 8, false, AROUND>); else run(pool_score_save_kernel<T, 4, false, AROUND>); }
+            else if (wide) run(pool_score_save_kernel<T, 8, true, AROUND>);
+            else run(pool_score_save_kernel<T, 4, true, AROUND>);
+        };
+        with_flag((long)frames * tokens_per_frame * D * (long)sizeof(T) > STREAM_BYTES, pick);
     });
     if (few) hipLaunchKernelGGL(pool_dot_kernel, dim3(frames), dim3(256), 0, s, pooled, ldp, D, w, b, logits);
     return launched();
@@ -208,8 +213,10 @@ extern "C" int vitg_pool_score_backward(const float* pooled, long ldp, int frame
     const bool wide = dh && dh_dtype != DT_F32 && D % 8 == 0 && lddh % 8 == 0 && aligned_to(dh, 16);
     with_dtype(dh ? dh_dtype : (int)DT_F32, [&](auto ti) {
         typedef decltype(ti) T;
-        if (wide) hipLaunchKernelGGL((pool_score_backward_kernel<T, 8>), dim3(grid), dim3(256), 0, (hipStream_t)stream, pooled, ldp, frames, tokens_per_frame, D, w, dlogits, (T*)dh, lddh, dw, db, accumulate, wblocks);
-        else hipLaunchKernelGGL((pool_score_backward_kernel<T, 4>), dim3(grid), dim3(256), 0, (hipStream_t)stream, pooled, ldp, frames, tokens_per_frame, D, w, dlogits, (T*)dh, lddh, dw, db, accumulate, wblocks);
+        auto run = [&](auto kernel) {
+            hipLaunchKernelGGL(kernel, dim3(grid), dim3(256), 0, (hipStream_t)stream, pooled, ldp, frames, tokens_per_frame, D, w, dlogits, (T*)dh, lddh, dw, db, accumulate, wblocks);
+        };
+        if (wide) run(pool_score_backward_kernel<T, 8>); else run(pool_score_backward_kernel<T, 4>);
     });
     return launched();
 }
