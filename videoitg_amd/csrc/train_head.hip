@@ -7,52 +7,68 @@
 //
 // The backward of the mean needs no second look at h: the forward keeps the frame means (frames x D fp32, 1 / tokens of h), so a step reads h once and
 // writes dh once - HBM-bound on both sides.
-#include <type_traits>
 #include "train_common.h"
 
 namespace vitg {
 
-// One block per frame when there are enough frames to fill the chip; otherwise the columns of a frame are spread over gridDim.y blocks (SCORE = false) and
-// pool_dot_kernel takes the scores from the means.
-template <typename T, int V, bool SCORE, bool AROUND>
+// rows j0 .. j1-1 of one frame, V columns, summed
+template <typename T, int V, bool AROUND>
+__device__ __forceinline__ void sum_rows(const T* __restrict__ p, long ldh, int j0, int j1, float (&s)[V]) {
+#pragma unroll
+    for (int e = 0; e < V; ++e) s[e] = 0.f;
+#pragma unroll 5
+    for (int j = j0; j < j1; ++j) {
+        float v[V];
+        load_stream<T, V, AROUND>(p + j * ldh, v);
+#pragma unroll
+        for (int e = 0; e < V; ++e) s[e] += v[e];
+    }
+}
+
+// one block per frame: enough frames to fill the chip
+template <typename T, int V, bool AROUND>
 __global__ __launch_bounds__(1024) void pool_score_save_kernel(const T* __restrict__ h, long ldh, int tokens, int cv, const float* __restrict__ w,
                                                                const float* __restrict__ b, float* __restrict__ logits, float* __restrict__ pooled, long ldp) {
+    __shared__ float part[16];
     const long t = blockIdx.x;
     const float inv = 1.0f / (float)tokens;
     float dot = 0.f;
-    for (int c = blockIdx.y * blockDim.x + threadIdx.x; c < cv; c += gridDim.y * blockDim.x) {
-        const T* const p = h + t * tokens * ldh + (long)c * V;
-        float s[V];
+    for (int c = threadIdx.x; c < cv; c += blockDim.x) {
+        float s[V], ww[V];
+        sum_rows<T, V, AROUND>(h + t * tokens * ldh + (long)c * V, ldh, 0, tokens, s);
+        load_vec<float, V>(w + c * V, ww);
 #pragma unroll
-        for (int e = 0; e < V; ++e) s[e] = 0.f;
-#pragma unroll 5
-        for (int j = 0; j < tokens; ++j) {
-            float v[V];
-            load_stream<T, V, AROUND>(p + j * ldh, v);
-#pragma unroll
-            for (int e = 0; e < V; ++e) s[e] += v[e];
-        }
-#pragma unroll
-        for (int e = 0; e < V; ++e) s[e] *= inv;
+        for (int e = 0; e < V; ++e) { s[e] *= inv; dot += s[e] * ww[e]; }
         store_vec<float, V>(pooled + t * ldp + (long)c * V, s);
-        if constexpr (SCORE) {
-            float ww[V];
-            load_vec<float, V>(w + c * V, ww);
+    }
+    dot = wave_sum(dot);
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = dot;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        float sum = 0.f;
+        for (int i = 0; i < (int)(blockDim.x >> 6); ++i) sum += part[i];
+        logits[t] = sum + b[0];
+    }
+}
+
+// fewer frames than CUs: a block takes 64 column groups of one frame, its four waves a quarter of the rows each (joined in order); pool_dot_kernel takes the
+// scores from the means
+template <typename T, int V, bool AROUND>
+__global__ __launch_bounds__(256) void pool_mean_kernel(const T* __restrict__ h, long ldh, int tokens, int cv, float* __restrict__ pooled, long ldp) {
+    __shared__ float part[3][64][V];
+    const long t = blockIdx.x;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = blockIdx.y * 64 + lane;
+    float s[V];
+    if (c < cv) {
+        sum_rows<T, V, AROUND>(h + t * tokens * ldh + (long)c * V, ldh, (int)((long)tokens * wave / 4), (int)((long)tokens * (wave + 1) / 4), s);
+        if (wave) store_vec<float, V>(part[wave - 1][lane], s);
+    }
+    __syncthreads();
+    if (wave || c >= cv) return;
+    const float inv = 1.0f / (float)tokens;
 #pragma unroll
-            for (int e = 0; e < V; ++e) dot += s[e] * ww[e];
-        }
-    }
-    if constexpr (SCORE) {
-        __shared__ float part[16];
-        dot = wave_sum(dot);
-        if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = dot;
-        __syncthreads();
-        if (threadIdx.x == 0) {
-            float sum = 0.f;
-            for (int i = 0; i < (int)(blockDim.x >> 6); ++i) sum += part[i];
-            logits[t] = sum + b[0];
-        }
-    }
+    for (int e = 0; e < V; ++e) s[e] = (((s[e] + part[0][lane][e]) + part[1][lane][e]) + part[2][lane][e]) * inv;
+    store_vec<float, V>(pooled + t * ldp + (long)c * V, s);
 }
 
 __global__ __launch_bounds__(256) void pool_dot_kernel(const float* __restrict__ pooled, long ldp, int D, const float* __restrict__ w, const float* __restrict__ b,
@@ -111,7 +127,8 @@ __global__ __launch_bounds__(1024) void bce_loss_backward_kernel(const float* __
     }
 }
 
-// blocks [0, wblocks): 64 columns of dw each (16 column quads x 16 frame groups) and, in block 0, db; the others: one frame of dh each
+// blocks [0, wblocks): 64 columns of dw each (16 column quads x 16 frame groups) and, in block 0, db; the others: up to DH_ROWS rows of one frame of dh each
+constexpr int DH_ROWS = 32;
 template <typename T, int V>
 __global__ __launch_bounds__(256) void pool_score_backward_kernel(const float* __restrict__ pooled, long ldp, int frames, int tokens, int D,
                                                                   const float* __restrict__ w, const float* __restrict__ dz, T* __restrict__ dh, long lddh,
@@ -151,14 +168,16 @@ __global__ __launch_bounds__(256) void pool_score_backward_kernel(const float* _
         }
         return;
     }
-    const long t = (int)blockIdx.x - wblocks;
+    const int slices = (tokens + DH_ROWS - 1) / DH_ROWS, id = (int)blockIdx.x - wblocks;
+    const long t = id / slices;
+    const int j0 = id % slices * DH_ROWS, j1 = min(j0 + DH_ROWS, tokens);
     const float d = dz[t] / (float)tokens;
     for (int c = threadIdx.x * V; c < D; c += 256 * V) {
         float v[V];
         load_vec<float, V>(w + c, v);
 #pragma unroll
         for (int e = 0; e < V; ++e) v[e] *= d;
-        for (int j = 0; j < tokens; ++j) store_vec<T, V>(dh + (t * tokens + j) * lddh + c, v);
+        for (int j = j0; j < j1; ++j) store_vec<T, V>(dh + (t * tokens + j) * lddh + c, v);
     }
 }
 
@@ -176,19 +195,18 @@ extern "C" int vitg_pool_score_save(const void* h, int h_dtype, long ldh, int fr
     const bool wide = h_dtype != DT_F32 && D % 8 == 0 && ldh % 8 == 0 && aligned_to(h, 16);
     const int cv = D / (wide ? 8 : 4);
     const bool few = frames < device_cu_count(current_device()) && tokens_per_frame >= 8 && cv > 64;
-    const int threads = few ? 64 : cv >= 1024 ? 1024 : (cv + 63) / 64 * 64;
-    const dim3 grid(frames, few ? ceil_div(cv, 64) : 1);
+    const int threads = cv >= 1024 ? 1024 : (cv + 63) / 64 * 64;
     hipStream_t s = (hipStream_t)stream;
     with_dtype(h_dtype, [&](auto ti) {
         typedef decltype(ti) T;
-        auto run = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(threads), 0, s, (const T*)h, ldh, tokens_per_frame, cv, w, b, logits, pooled, ldp); };
-        auto pick = [&](auto around) {
+        with_flag((long)frames * tokens_per_frame * D * (long)sizeof(T) > STREAM_BYTES, [&](auto around) {
             constexpr bool AROUND = decltype(around)::value;
-            if (few) { if (wide) run(pool_score_save_kernel<T, 8, false, AROUND>); else run(pool_score_save_kernel<T, 4, false, AROUND>); }
-            else if (wide) run(pool_score_save_kernel<T, 8, true, AROUND>);
-            else run(pool_score_save_kernel<T, 4, true, AROUND>);
-        };
-        with_flag((long)frames * tokens_per_frame * D * (long)sizeof(T) > STREAM_BYTES, pick);
+            auto mean = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(frames, ceil_div(cv, 64)), dim3(256), 0, s, (const T*)h, ldh, tokens_per_frame, cv, pooled, ldp); };
+            auto all = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(frames), dim3(threads), 0, s, (const T*)h, ldh, tokens_per_frame, cv, w, b, logits, pooled, ldp); };
+            if (few) { if (wide) mean(pool_mean_kernel<T, 8, AROUND>); else mean(pool_mean_kernel<T, 4, AROUND>); }
+            else if (wide) all(pool_score_save_kernel<T, 8, AROUND>);
+            else all(pool_score_save_kernel<T, 4, AROUND>);
+        });
     });
     if (few) hipLaunchKernelGGL(pool_dot_kernel, dim3(frames), dim3(256), 0, s, pooled, ldp, D, w, b, logits);
     return launched();
@@ -208,8 +226,10 @@ extern "C" int vitg_pool_score_backward(const float* pooled, long ldp, int frame
     if ((dh && lddh < D) || (dw && frames && ldp < D)) return VITG_ERR_SHAPE;
     if (D % 4 || !aligned_to(w, 16) || (dw && (ldp % 4 || !aligned_to(pooled, 16))) || (dh && (lddh % 4 || !aligned_to(dh, 4 * dtype_size(dh_dtype))))) return VITG_ERR_ALIGN;
     const int wblocks = dw ? ceil_div(D, 64) : db ? 1 : 0;
-    const unsigned grid = (unsigned)wblocks + (unsigned)(dh ? frames : 0);
-    if (!grid) return 0;
+    const long blocks = wblocks + (dh ? (long)frames * ceil_div(tokens_per_frame, DH_ROWS) : 0);
+    if (!blocks) return 0;
+    if (blocks >= (1l << 31)) return VITG_ERR_SHAPE;
+    const unsigned grid = (unsigned)blocks;
     const bool wide = dh && dh_dtype != DT_F32 && D % 8 == 0 && lddh % 8 == 0 && aligned_to(dh, 16);
     with_dtype(dh ? dh_dtype : (int)DT_F32, [&](auto ti) {
         typedef decltype(ti) T;
