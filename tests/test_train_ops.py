@@ -14,9 +14,10 @@ U32 = 2.0 ** -24
 
 
 def within(got, want, bound):
-    """|got - want| <= bound elementwise (64 bits, on the host); NaN nowhere"""
-    got, want = got.detach().double().cpu(), want.double().cpu()
-    bound = bound.double().cpu() if torch.is_tensor(bound) else torch.full_like(want, bound)
+    """|got - want| <= bound elementwise (64 bits, where `want` is); NaN nowhere"""
+    want = want.double()
+    got = got.detach().to(want.device).double()
+    bound = bound.double().to(want.device) if torch.is_tensor(bound) else torch.full_like(want, bound)
     bad = ~((got - want).abs() <= bound)
     assert not bad.any(), (f"{int(bad.sum())} of {bad.numel()} outside the bound, worst by "
                            f"{float(((got - want).abs() / bound.clamp_min(1e-300)).nan_to_num(float('inf')).max()):.3g}")
@@ -172,16 +173,26 @@ FFN_SHAPES = [(1, 64, 64), (2, 128, 192), (16, 192, 320), (17, 256, 1216), (64, 
               (400, 256, 832), (1000, 128, 1984)]
 
 
+# shapes that reach the other kernels (256 CUs: at most one 128x128 tile each is the ring kernel's case): 128x128 tiles at two per CU, 256-, 320- and 384-row tiles
+FFN_WIDE = [(100, 64, 33024), (200, 64, 16576), (300, 64, 12800), (300, 64, 25600), (400, 128, 12864), (1000, 64, 16384), (770, 192, 24640)]
+
+
+def place(*tensors):
+    """the reference's operands, 64 bits, on the device (the host would take minutes over the wide shapes)"""
+    return [t.cuda().double() for t in tensors]
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [BF16, F16])
-@pytest.mark.parametrize("m,k,n", FFN_SHAPES)
+@pytest.mark.parametrize("m,k,n", FFN_SHAPES + FFN_WIDE)
 @pytest.mark.parametrize("extra", [0, 8])
 def test_swiglu(ops, dtype, m, k, n, extra):
     x, w = randn(m, k, dtype=dtype), randn(n, k, dtype=dtype, scale=k ** -0.5 * 1.5)
     out, gu = strided(torch.zeros(m, n // 2, dtype=dtype), extra), strided(torch.zeros(m, n, dtype=dtype), extra)
     ops.swiglu(strided(x, extra), strided(w, extra), out, gu=gu)
-    pre = x.double() @ w.double().t()
-    err = k * 2.0 ** -23 * (x.double().abs() @ w.double().abs().t())                   # the fp32 sums
+    x64, w64 = place(x, w)
+    pre = x64 @ w64.t()
+    err = k * 2.0 ** -23 * (x64.abs() @ w64.abs().t())                                 # the fp32 sums
     within(gu, pre, err + HALF[dtype] * (pre.abs() + err) * 1.001 + TINY[dtype])
     (gate, up), (eg, eu) = halves(pre), halves(err)
     silu = gate * torch.sigmoid(gate)
@@ -198,11 +209,49 @@ def test_swiglu(ops, dtype, m, k, n, extra):
 
 
 def ffn_grads(dout, gu, x, w):
-    """64-bit gradients from the saved pre-activations, and the sums of magnitudes behind them"""
-    gate, up = halves(gu.double())
-    d, sig = dout.double(), torch.sigmoid(gate)
-    dgu = interleave(d * up * sig * (1 + gate * (1 - sig)), d * gate * sig)
-    return dgu, dgu @ w.double(), dgu.t() @ x.double(), dgu.abs() @ w.double().abs(), dgu.abs().t() @ x.double().abs()
+    """gradients in 64 bits from the saved pre-activations, and the sums of magnitudes behind them"""
+    gate, up = halves(gu)
+    sig = torch.sigmoid(gate)
+    dgu = interleave(dout * up * sig * (1 + gate * (1 - sig)), dout * gate * sig)
+    return dgu, dgu @ w, dgu.t() @ x, dgu.abs() @ w.abs(), dgu.abs().t() @ x.abs()
+
+
+def check_swiglu_backward(ops, dtype, m, k, n, dw_kind, extra):
+    x, w = randn(m, k, dtype=dtype), randn(n, k, dtype=dtype, scale=k ** -0.5)
+    gu, dout = randn(m, n, dtype=dtype, scale=1.3, seed=1), randn(m, n // 2, dtype=dtype, scale=0.3, seed=2)
+    dw_dtype = F32 if dw_kind.startswith("fp32") else dtype
+    old = randn(n, k, dtype=dw_dtype, scale=0.7, seed=4)
+    add = dw_kind.endswith("add")
+    dx, dw = strided(torch.zeros(m, k, dtype=dtype), extra), strided(old, extra)
+    ops.swiglu_backward(strided(dout, extra), strided(gu, extra), strided(x, extra), strided(w, extra), dx=dx, dw=dw, accumulate=add)
+    dout64, gu64, x64, w64, old64 = place(dout, gu, x, w, old)
+    dgu, want_x, want_w, mass_x, mass_w = ffn_grads(dout64, gu64, x64, w64)
+    # dGU in 32 bits (2^-18 of the value: exponential, reciprocal, five products and 1 + G (1 - sig), whose cancellation is at most 4.6 in magnitude of its
+    # terms over its value where dG matters; taken on the magnitude of dH U sig (1 + |G|)), then one rounding to the operand type, then the fp32 sums
+    gate, up = halves(gu64)
+    sig = torch.sigmoid(gate)
+    fuzz = interleave((dout64 * up).abs() * sig * (1 + gate.abs()), (dout64 * gate).abs() * sig) * 2.0 ** -18 + TINY[dtype]
+    ex = (HALF[dtype] * 1.01 + n * 2.0 ** -23) * mass_x + fuzz @ w64.abs()
+    ew = (HALF[dtype] * 1.01 + m * 2.0 ** -23) * mass_w + fuzz.t() @ x64.abs()
+    if add:
+        want_w = want_w + old64
+        ew = ew + m * 2.0 ** -23 * old64.abs()
+    within(dx, want_x, ex + HALF[dtype] * (want_x.abs() + ex) + TINY[dtype])
+    within(dw, want_w, ew + HALF[dw_dtype] * (want_w.abs() + ew) + TINY[dw_dtype])
+    # independent roundings average: over the whole matrix the error is far below the worst case
+    assert (dx.double() - want_x).norm() <= 2 * HALF[dtype] * want_x.norm()
+    assert (dw.double() - want_w).norm() <= 2 * HALF[dtype] * want_w.norm()
+    if extra:
+        assert (torch.as_strided(dx, (m, extra), (k + extra, 1), k) == 7.0).all() and (torch.as_strided(dw, (n, extra), (k + extra, 1), k) == 7.0).all()
+    # each alone, where another split or kernel may take it
+    only_x, only_w = torch.empty(m, k, dtype=dtype, device="cuda"), old.cuda().clone()
+    ops.swiglu_backward(dout.cuda(), gu.cuda(), x.cuda(), w.cuda(), dx=only_x)
+    ops.swiglu_backward(dout.cuda(), gu.cuda(), x.cuda(), w.cuda(), dw=only_w, accumulate=add)
+    within(only_x, want_x, ex + HALF[dtype] * (want_x.abs() + ex) + TINY[dtype])
+    within(only_w, want_w, ew + HALF[dw_dtype] * (want_w.abs() + ew) + TINY[dw_dtype])
+    again = torch.empty(m, k, dtype=dtype, device="cuda")
+    ops.swiglu_backward(dout.cuda(), gu.cuda(), x.cuda(), w.cuda(), dx=again)
+    assert torch.equal(again, only_x)                                                  # a fixed summation order
 
 
 @pytest.mark.gpu
@@ -210,36 +259,17 @@ def ffn_grads(dout, gu, x, w):
 @pytest.mark.parametrize("m,k,n", FFN_SHAPES + [(129, 1024, 4096), (300, 256, 8192), (33, 576, 1024), (2100, 64, 128), (3000, 320, 192), (5000, 512, 64)])
 @pytest.mark.parametrize("dw_kind", ["same", "same_add", "fp32", "fp32_add"])
 def test_swiglu_backward(ops, dtype, m, k, n, dw_kind):
-    x, w = randn(m, k, dtype=dtype), randn(n, k, dtype=dtype, scale=k ** -0.5)
-    gu, dout = randn(m, n, dtype=dtype, scale=1.3, seed=1), randn(m, n // 2, dtype=dtype, scale=0.3, seed=2)
-    dw_dtype = F32 if dw_kind.startswith("fp32") else dtype
-    old = randn(n, k, dtype=dw_dtype, scale=0.7, seed=4)
-    add = dw_kind.endswith("add")
-    extra = 8 if m % 2 else 0
-    dx, dw = strided(torch.zeros(m, k, dtype=dtype), extra), strided(old, extra)
-    ops.swiglu_backward(strided(dout, extra), strided(gu, extra), strided(x, extra), strided(w, extra), dx=dx, dw=dw, accumulate=add)
-    dgu, want_x, want_w, mass_x, mass_w = ffn_grads(dout, gu, x, w)
-    # dGU in 32 bits (2^-18 of the value: exponential, reciprocal, five products and 1 + G (1 - sig), whose cancellation is at most 4.6 in magnitude of its
-    # terms over its value where dG matters; taken on the magnitude of dH U sig (1 + |G|)), then one rounding to the operand type, then the fp32 sums
-    gate, up = halves(gu.double())
-    sig = torch.sigmoid(gate)
-    fuzz = interleave((dout.double() * up).abs() * sig * (1 + gate.abs()), (dout.double() * gate).abs() * sig) * 2.0 ** -18 + TINY[dtype]
-    ex = (HALF[dtype] * 1.01 + n * 2.0 ** -23) * mass_x + fuzz @ w.double().abs()
-    ew = (HALF[dtype] * 1.01 + m * 2.0 ** -23) * mass_w + fuzz.t() @ x.double().abs()
-    if add:
-        want_w = want_w + old.double()
-        ew = ew + m * 2.0 ** -23 * old.double().abs()
-    within(dx, want_x, ex + HALF[dtype] * (want_x.abs() + ex) + TINY[dtype])
-    within(dw, want_w, ew + HALF[dw_dtype] * (want_w.abs() + ew) + TINY[dw_dtype])
-    # independent roundings average: over the whole matrix the error is far below the worst case
-    rel = (dx.double().cpu() - want_x).norm() / want_x.norm()
-    assert rel <= 2 * HALF[dtype], rel
-    if extra:
-        assert (torch.as_strided(dx, (m, extra), (k + extra, 1), k) == 7.0).all() and (torch.as_strided(dw, (n, extra), (k + extra, 1), k) == 7.0).all()
-    only_x, only_w = torch.empty(m, k, dtype=dtype, device="cuda"), old.cuda().clone()
-    ops.swiglu_backward(dout.cuda(), gu.cuda(), x.cuda(), w.cuda(), dx=only_x)
-    ops.swiglu_backward(dout.cuda(), gu.cuda(), x.cuda(), w.cuda(), dw=only_w, accumulate=add)
-    assert torch.equal(only_x, dx) and torch.equal(only_w, dw)                         # each alone: the same bits
+    check_swiglu_backward(ops, dtype, m, k, n, dw_kind, 8 if m % 2 else 0)
+
+
+# wider layers (256 CUs): W as it lies on 256- and 320-row tiles, whole and split; W transposed, whole (256- and 384-row tiles) and split (256, 320); dW whole
+# and split on 256x256 tiles; the ring kernel on one of the two products only
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,k,n", [(2100, 2048, 128), (2100, 2048, 1024), (300, 3584, 8192), (700, 4096, 6144), (4100, 2048, 2560), (3463, 320, 41344), (3177, 320, 51648),
+                                   (7000, 1088, 2048), (734, 192, 16896), (900, 2048, 4096), (100, 2048, 16576), (20, 1088, 20544)])
+@pytest.mark.parametrize("dtype,dw_kind", [(BF16, "same"), (F16, "fp32_add"), (BF16, "same_add")])
+def test_swiglu_backward_wide(ops, dtype, m, k, n, dw_kind):
+    check_swiglu_backward(ops, dtype, m, k, n, dw_kind, 8 if m % 3 == 0 else 0)
 
 
 @pytest.mark.gpu

@@ -723,12 +723,18 @@ def embed_lookup(ids: torch.Tensor, table: torch.Tensor, out: torch.Tensor, *, s
     return out
 
 
-@functools.lru_cache(maxsize=1024)
 def embed_backward_plan(n: int, d: int) -> int:
     """workspace bytes of embed_backward for n tokens of width d"""
     b = C.c_long(0)
     _lib.call("vitg_embed_backward_plan", n, d, C.byref(b))
     return b.value
+
+
+@functools.lru_cache(maxsize=4096)
+def _plan_on(idx: int, plan, *args) -> int:
+    """a plan on device idx (it depends on the sizes and the device alone)"""
+    with torch.cuda.device(idx):
+        return plan(*args)
 
 
 def embed_backward(ids: torch.Tensor, dout: torch.Tensor, dtable: torch.Tensor, *, scale: float = 1.0, accumulate: bool = False,
@@ -740,7 +746,7 @@ def embed_backward(ids: torch.Tensor, dout: torch.Tensor, dtable: torch.Tensor, 
     pi, ei = _vector(ids, "ids", n, torch.int64)
     pd, ldd, ed = _matrix(dout, "dout", n, d, _FLOATS)
     pt, ldt, et = _matrix(dtable, "dtable", vocab, d, _FLOATS)
-    ws, pw, nw = _workspace(workspace, embed_backward_plan(n, d), idx)
+    ws, pw, nw = _workspace(workspace, _plan_on(idx, embed_backward_plan, n, d), idx)
     _distinct([("dtable", pt, et), ("workspace", pw, pw + nw)], [("dout", pd, ed), ("ids", pi, ei)])
     _call_on(idx, "vitg_embed_backward", pi, n, pd, _DT[dout.dtype], ldd, vocab, d, scale, pt, _DT[dtable.dtype], ldt, 1 if accumulate else 0, pw, nw)
     return dtable
@@ -764,9 +770,8 @@ def swiglu(x: torch.Tensor, w: torch.Tensor, out: torch.Tensor, *, gu: Optional[
     return out
 
 
-@functools.lru_cache(maxsize=1024)
 def swiglu_backward_plan(m: int, n: int, k: int, want_dx: bool = True, want_dw: bool = True) -> int:
-    """workspace bytes of swiglu_backward for x [m, k] and w [n, k]"""
+    """workspace bytes of swiglu_backward for x [m, k] and w [n, k] on the current device"""
     b = C.c_long(0)
     _lib.call("vitg_swiglu_backward_plan", m, n, k, int(want_dx), int(want_dw), C.byref(b))
     return b.value
@@ -793,7 +798,7 @@ def swiglu_backward(dout: torch.Tensor, gu: torch.Tensor, x: torch.Tensor, w: to
         outs.append(("dw", pdw, e))
     if not outs:
         return
-    ws, pws, nws = _workspace(workspace, swiglu_backward_plan(m, nn, k, dx is not None, dw is not None), idx)
+    ws, pws, nws = _workspace(workspace, _plan_on(idx, swiglu_backward_plan, m, nn, k, dx is not None, dw is not None), idx)
     outs.append(("workspace", pws, pws + nws))
     _distinct(outs, (("dout", pd, ed), ("gu", pg, eg), ("x", px, ex), ("w", pw, ew)))
     _call_on(idx, "vitg_swiglu_backward", pd, ldd, pg, ldg, px, ldx, pw, ldw, m, nn, k, _DT[dt], pdx, lddx, pdw, lddw, _DT[dwt], 1 if accumulate else 0, pws, nws)
