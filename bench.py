@@ -760,14 +760,11 @@ def bench_videos(args, cfg, eng, dtype, dev, rank, world, T, R):
 
 
 def spawn_ranks(n: int) -> None:
-    """`python bench.py --gpus N` without a launcher: run this command line under torch's elastic launcher - one process per GPU
+    """`python bench.py --gpus N` without a launcher: re-execute this command line under torch's elastic launcher - one process per GPU
     on this node, rendezvous on 127.0.0.1 and a free port - which is what the reference's `accelerate launch --num_processes=8`
-    (/root/reference/scripts/eval_lmms_eval/videomme_grounding.sh:3-5) does for its own per-GPU processes.  A child process (this one has
-    asked for the devices already, and a process that has touched the GPU is not replaced) on the same stdout, where the JSON line of rank 0 is
-    the only thing printed; this process passes SIGTERM / SIGINT on and ends with the launcher's status."""
-    import signal
+    (/root/reference/scripts/eval_lmms_eval/videomme_grounding.sh:3-5) does for its own per-GPU processes.  exec: same PID, same stdout,
+    the JSON line of rank 0 is the only thing printed there."""
     import socket
-    import subprocess
     s = socket.socket()
     s.bind(("127.0.0.1", 0))
     port = s.getsockname()[1]
@@ -777,10 +774,7 @@ def spawn_ranks(n: int) -> None:
     cmd = [sys.executable, "-m", "torch.distributed.run", "--nnodes=1", f"--nproc-per-node={n}", "--master-addr", "127.0.0.1",
            "--master-port", str(port), os.path.abspath(__file__)] + sys.argv[1:]
     sys.stdout.flush()
-    child = subprocess.Popen(cmd)
-    for sig in (signal.SIGTERM, signal.SIGINT):
-        signal.signal(sig, lambda number, frame: child.send_signal(number))
-    sys.exit(child.wait())
+    os.execv(sys.executable, cmd)
 
 
 def main():
