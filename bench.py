@@ -786,7 +786,8 @@ def main():
     backend_asked = os.environ.get("VITG_DIST_BACKEND", "nccl")        # "nccl" = RCCL over xGMI
     if world != args.gpus:
         if "WORLD_SIZE" not in os.environ and args.gpus > 1:
-            why = preflight_ranks(args.gpus, torch.cuda.device_count() if torch.cuda.is_available() else 0, backend_asked, single_device)
+            # the count alone (0 without a GPU): it leaves the devices untouched, so this process may still be replaced by the launcher
+            why = preflight_ranks(args.gpus, torch.cuda.device_count(), backend_asked, single_device)
             if why:                                     # before any rank is started: the launcher never sees a half-started job
                 sys.exit(f"bench.py: {why}")
             return spawn_ranks(args.gpus)               # plain `python bench.py --gpus N`: this process becomes the launcher of its N ranks
