@@ -520,6 +520,67 @@ def test_training_step_in_a_graph_and_on_another_stream(ops):
             assert torch.equal(out[n], eager[n]), n
 
 
+@pytest.mark.gpu
+def test_given_workspaces_of_exactly_the_planned_size(ops):
+    for m, k, n in ((5, 128, 256), (300, 256, 832), (2100, 2048, 128)):
+        x, w, gu, dout = (randn(*s, dtype=F16, seed=i).cuda() for i, s in enumerate(((m, k), (n, k), (m, n), (m, n // 2))))
+        need = ops.swiglu_backward_plan(m, n, k)
+        guard = torch.full((need + 4096,), 0x5a, dtype=torch.uint8, device="cuda")
+        got, want = [torch.empty_like(x), torch.empty_like(w)], [torch.empty_like(x), torch.empty_like(w)]
+        ops.swiglu_backward(dout, gu, x, w, dx=got[0], dw=got[1], workspace=guard[:need])
+        ops.swiglu_backward(dout, gu, x, w, dx=want[0], dw=want[1])
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]) and (guard[need:] == 0x5a).all()
+    for t, d in ((37, 36), (20000, 24)):
+        ids, rows = torch.randint(0, 50, (t,), device="cuda"), randn(t, d).cuda()
+        need = ops.embed_backward_plan(t, d)
+        guard = torch.full((need + 4096,), 0x5a, dtype=torch.uint8, device="cuda")
+        got = ops.embed_backward(ids, rows, torch.empty(50, d, device="cuda"), workspace=guard[:need])
+        assert torch.equal(got, ops.embed_backward(ids, rows, torch.empty(50, d, device="cuda"))) and (guard[need:] == 0x5a).all()
+    grads = [randn(70000, seed=i).cuda() for i in range(100)]
+    guard = torch.full((2 * 1024 * 8 + 4096,), 0x5a, dtype=torch.uint8, device="cuda")      # two launches' sums: 96 + 4 tensors of 5 pieces
+    need = (96 * 5 + 4 * 5) * 8
+    norm = torch.zeros(1, device="cuda")
+    assert ops.clip_grad_norm(grads, None, norm=norm, workspace=guard[:need]) is norm
+    assert torch.equal(norm, ops.clip_grad_norm(grads, None)) and (guard[need:] == 0x5a).all()
+
+
+@pytest.mark.gpu
+def test_calls_on_two_streams_at_once(ops):
+    """the same operators on other data on two streams, without a wait in between: each result is its own"""
+    from videoitg_amd.torch_ops import K
+    steps = [Step(BF16, frames=40, tokens=9, k=256, f=192, vocab=300, seed=s) for s in (11, 12)]
+    want = [{n: t.clone() for n, t in st.run(K).items()} for st in steps]
+    streams = [torch.cuda.Stream() for _ in steps]
+    torch.cuda.synchronize()
+    got = [None, None]
+    for _ in range(3):
+        for i, (st, stream) in enumerate(zip(steps, streams)):
+            with torch.cuda.stream(stream):
+                got[i] = st.run(K)
+    torch.cuda.synchronize()
+    for w, g in zip(want, got):
+        for n in w:
+            assert torch.equal(w[n], g[n]), n
+
+
+@pytest.mark.gpu
+def test_dispatcher_forms_equal_the_binding(ops):
+    from videoitg_amd.torch_ops import K
+    grads = [randn(4000, dtype=F16, seed=1).cuda(), randn(33, seed=2).cuda()]
+    outs, want = [torch.empty_like(t) for t in grads], [torch.empty_like(t) for t in grads]
+    norm = K.clip_grad_norm(grads, 0.5, outs=outs, scale=0.5)
+    assert torch.equal(norm, ops.clip_grad_norm(grads, 0.5, outs=want, scale=0.5)) and all(torch.equal(a, b) for a, b in zip(outs, want))
+    assert torch.equal(K.clip_grad_norm(grads, None), ops.clip_grad_norm(grads, None))
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    with FakeTensorMode():
+        z = torch.empty(7, device="cuda")
+        loss, weight, dz = torch.ops.videoitg.bce_loss_backward(z, z)
+        assert loss.shape == () and weight.shape == () and dz.shape == (7,)
+        assert torch.ops.videoitg.grad_norm([z]).shape == (1,)
+    with pytest.raises(NotImplementedError):
+        torch.ops.videoitg.embed_lookup(torch.zeros(1, dtype=torch.int64), torch.zeros(2, 4), torch.zeros(1, 4))
+
+
 # ---- refusals ------------------------------------------------------------------------------------------------------------------------------
 @pytest.fixture(scope="module")
 def lib():
