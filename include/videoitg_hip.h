@@ -299,7 +299,7 @@ int vitg_attention_split(const void* q, const void* k, const void* v, void* o, l
  *   a zero row.  D, ldt, ldo multiples of 4.  (vitg_embed_gather without a scale, bounds or other types.)  embed_tokens at eagle/model/eagle_archv1.py:310.
  * vitg_embed_backward: dtable[v, :] = scale * sum over i with ids[i] = v of dout[i, :] for EVERY v < vocab (accumulate = 0: rows without a token are zero), or
  *   dtable[v, :] += that sum for the rows of the batch only (accumulate = 1).  ids outside the vocabulary contribute nothing.  fp32 sums.  Columns D .. ldt-1
- *   keep their contents.  workspace: vitg_embed_backward_plan bytes, 16-byte aligned. */
+ *   keep their contents.  At most 2^24 tokens a call.  workspace: vitg_embed_backward_plan bytes, 16-byte aligned. */
 int vitg_embed_lookup(const long long* ids, long n, const void* table, int table_dtype, long ldt, long vocab, int D, float scale, void* out, int out_dtype,
                       long ldo, void* stream);
 int vitg_embed_backward_plan(long n, int D, long* workspace_bytes);
@@ -320,10 +320,10 @@ int vitg_swiglu_backward(const void* dout, int lddo, const void* gu, int ldgu, c
 
 /* The score head and grounding loss (grounding_qwen2.py:148-169) with their gradients.
  * vitg_pool_score_save: vitg_pool_score on fp32 / fp16 / bf16 rows (row t * tokens_per_frame + j, leading dimension ldh), keeping the frame means
- *   pooled[frames, ldp] (fp32).
+ *   pooled[frames, ldp] (fp32).  Fewer than 2^22 frames.
  * vitg_bce_loss_backward: vitg_bce_loss (out2 = loss, pos_weight) and dlogits = scale * d loss / d logits.
  * vitg_pool_score_backward: dh[t * tokens_per_frame + j, :] = dlogits[t] / tokens_per_frame * w (fp32 / fp16 / bf16), dw (+)= sum_t dlogits[t] pooled[t, :],
- *   db (+)= sum_t dlogits[t]; each of dh / dw / db may be NULL; accumulate applies to dw and db. */
+ *   db (+)= sum_t dlogits[t]; each of dh / dw / db may be NULL; accumulate applies to dw and db.  Fewer than 2^24 slices of 32 tokens over all frames. */
 int vitg_pool_score_save(const void* h, int h_dtype, long ldh, int frames, int tokens_per_frame, int D, const float* w, const float* b, float* logits,
                          float* pooled, long ldp, void* stream);
 int vitg_bce_loss_backward(const float* logits, const float* labels, int n, float scale, float* out2, float* dlogits, void* stream);

@@ -149,6 +149,19 @@ def test_embed_backward_long_lists(ops, n, vocab, kind):
 
 
 @pytest.mark.gpu
+def test_embeddings_of_millions_of_tokens(ops):
+    """more rows than the lookup has blocks; a sort of thousands of tiles.  Whole numbers: every sum is exact in any order"""
+    n, d, vocab = 4_300_000, 4, 300_000
+    ids = torch.randint(-1, vocab, (n,), generator=torch.Generator().manual_seed(5)).cuda()
+    table = torch.randint(-8, 9, (vocab, d), generator=torch.Generator().manual_seed(6)).to(F16).cuda()
+    want = torch.where(ids[:, None] >= 0, table[ids.clamp(min=0)], torch.zeros((), dtype=F16, device="cuda"))
+    assert torch.equal(ops.embed_lookup(ids, table, torch.full((n, d), 7.0, dtype=F16, device="cuda")), want)
+    grad = torch.zeros(vocab + 1, d, dtype=torch.float64, device="cuda").index_add_(0, torch.where(ids >= 0, ids, vocab), want.double() + 1)[:vocab]
+    got = ops.embed_backward(ids, want.float() + 1, torch.empty(vocab, d, device="cuda"))
+    assert torch.equal(got.double(), grad)
+
+
+@pytest.mark.gpu
 def test_embed_backward_of_no_tokens(ops):
     table = torch.full((10, 8), 2.0, device="cuda")
     none, rows = torch.empty(0, dtype=torch.int64, device="cuda"), torch.empty(0, 8, device="cuda")
@@ -605,6 +618,7 @@ def test_embed_entries_refuse(lib):
     need = C.c_long(-1)
     assert lib.vitg_embed_backward_plan(0, 8, C.byref(need)) == 0 and need.value == 0
     assert lib.vitg_embed_backward_plan(100, 8, C.byref(need)) == 0 and need.value > 100 * 16
+    assert lib.vitg_embed_backward_plan((1 << 24) + 1, 8, C.byref(need)) == SHAPE and lib.vitg_embed_backward_plan(1 << 24, 8, C.byref(need)) == 0
     assert lib.vitg_embed_backward_plan(-1, 8, C.byref(need)) == SHAPE and lib.vitg_embed_backward_plan(4, 8, None) == ARG
     assert lib.vitg_embed_backward_plan(4, 8, C.byref(need)) == 0
 
@@ -612,6 +626,7 @@ def test_embed_entries_refuse(lib):
         return lib.vitg_embed_backward(ids, n, dout, ddt, ldd, vocab, d, 1.0, table, tdt, ldt, 0, ws, bytes_, NUL)
     assert back(table=NUL) == ARG and back(ids=NUL) == ARG and back(dout=NUL) == ARG and back(ws=NUL) == ARG and back(bytes_=need.value - 1) == ARG
     assert back(ddt=7) == DTYPE and back(tdt=7) == DTYPE
+    assert back(n=(1 << 24) + 1) == SHAPE
     assert back(n=-1) == SHAPE and back(vocab=0) == SHAPE and back(ldd=4) == SHAPE and back(ldt=4) == SHAPE and back(vocab=1 << 31) == SHAPE
     assert back(d=6) == ALIGN and back(ldd=10) == ALIGN and back(ldt=10) == ALIGN and back(table=ODD) == ALIGN and back(dout=ODD) == ALIGN and back(ws=ODD) == ARG
 
@@ -623,6 +638,7 @@ def test_swiglu_entries_refuse(lib):
     assert fwd(x=NUL) == ARG and fwd(w=NUL) == ARG and fwd(out=NUL) == ARG
     assert fwd(dt=2) == DTYPE
     assert fwd(k=32) == SHAPE and fwd(n=96) == SHAPE and fwd(ldx=56) == SHAPE and fwd(ldo=56) == SHAPE and fwd(ldgu=120) == SHAPE and fwd(ldw=1 << 22) == SHAPE
+    assert fwd(m=(1 << 31) - 1) == SHAPE and fwd(n=1 << 30, ldo=1 << 29, ldgu=1 << 30) == SHAPE
     assert fwd(ldx=68) == ALIGN and fwd(ldgu=132) == ALIGN and fwd(x=ODD) == ALIGN and fwd(gu=ODD) == ALIGN
 
     need = C.c_long(-1)
@@ -643,6 +659,7 @@ def test_head_and_clip_entries_refuse(lib):
         return lib.vitg_pool_score_save(h, dt, ldh, frames, tokens, d, w, b, logits, pooled, ldp, NUL)
     assert save(frames=0, h=NUL) == 0
     assert save(h=NUL) == ARG and save(pooled=NUL) == ARG and save(dt=5) == DTYPE and save(tokens=0) == SHAPE and save(ldh=4) == SHAPE
+    assert save(frames=1 << 22) == SHAPE
     assert save(d=6) == ALIGN and save(w=ODD) == ALIGN and save(ldp=10) == ALIGN
     assert lib.vitg_bce_loss_backward(P, P, 0, 1.0, P, P, NUL) == ARG and lib.vitg_bce_loss_backward(P, P, 3, 1.0, P, NUL, NUL) == ARG
 
@@ -650,6 +667,7 @@ def test_head_and_clip_entries_refuse(lib):
         return lib.vitg_pool_score_backward(pooled, ldp, frames, tokens, d, w, dz, dh, dt, lddh, dw, db, 0, NUL)
     assert back(dh=NUL, dw=NUL, db=NUL) == 0
     assert back(pooled=NUL) == ARG and back(w=NUL) == ARG and back(dz=NUL) == ARG and back(dt=4) == DTYPE and back(tokens=0) == SHAPE and back(frames=-1) == SHAPE
+    assert back(frames=1 << 24, tokens=1) == SHAPE and back(frames=1, tokens=(1 << 31) - 1, dw=NUL, db=NUL) == SHAPE
     assert back(lddh=4) == SHAPE and back(ldp=4) == SHAPE and back(d=6) == ALIGN and back(dh=ODD) == ALIGN
 
     one, f32 = (C.c_long * 1)(5), (C.c_int * 1)(2)

@@ -431,7 +431,7 @@ extern "C" int vitg_swiglu(const void* X, int ldx, const void* W, int ldw, int M
     if (!X || !W || !out) return VITG_ERR_ARG;
     if (dtype != DT_BF16 && dtype != DT_F16) return VITG_ERR_DTYPE;
     if (K <= 0 || K % 64 || N % 64 || ldx < K || ldw < K || ldo < N / 2 || (gu && ldgu < N)) return VITG_ERR_SHAPE;
-    if (!ld_ok(ldx) || !ld_ok(ldw) || !ld_ok(ldo) || (gu && !ld_ok(ldgu))) return VITG_ERR_SHAPE;
+    if (M >= (1 << 30) || N >= (1 << 30) || !ld_ok(ldx) || !ld_ok(ldw) || !ld_ok(ldo) || (gu && !ld_ok(ldgu))) return VITG_ERR_SHAPE;
     if (ldx % 8 || ldw % 8 || ldo % 8 || (gu && ldgu % 8)) return VITG_ERR_ALIGN;
     if (!aligned_to(X, 16) || !aligned_to(W, 16) || !aligned_to(out, 16) || (gu && !aligned_to(gu, 16))) return VITG_ERR_ALIGN;
     hipStream_t s = (hipStream_t)stream;

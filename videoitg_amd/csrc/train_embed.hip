@@ -14,23 +14,24 @@ namespace vitg {
 template <typename TI, typename TO, int V>
 __global__ void embed_lookup_kernel(const long long* __restrict__ ids, long n, const TI* __restrict__ table, long ldt, long vocab, int cv, float scale,
                                     TO* __restrict__ out, long ldo) {
-    const long row = (long)blockIdx.x * blockDim.y + threadIdx.y;
-    if (row >= n) return;
-    const long long id = ids[row];
-    const bool known = id >= 0 && id < vocab;
-    for (int c = threadIdx.x; c < cv; c += blockDim.x) {
-        float v[V];
-        if (known) {
-            load_vec<TI, V>(table + id * ldt + (long)c * V, v);
+    for (long row = (long)blockIdx.x * blockDim.y + threadIdx.y; row < n; row += (long)gridDim.x * blockDim.y) {
+        const long long id = ids[row];
+        const bool known = id >= 0 && id < vocab;
+        for (int c = threadIdx.x; c < cv; c += blockDim.x) {
+            float v[V];
+            if (known) {
+                load_vec<TI, V>(table + id * ldt + (long)c * V, v);
 #pragma unroll
-            for (int e = 0; e < V; ++e) v[e] *= scale;
-        } else {
+                for (int e = 0; e < V; ++e) v[e] *= scale;
+            } else {
 #pragma unroll
-            for (int e = 0; e < V; ++e) v[e] = 0.f;
+                for (int e = 0; e < V; ++e) v[e] = 0.f;
+            }
+            store_vec<TO, V>(out + row * ldo + (long)c * V, v);
         }
-        store_vec<TO, V>(out + row * ldo + (long)c * V, v);
     }
 }
+constexpr long LOOKUP_BLOCKS = 1l << 20;                 // (a launch has fewer than 2^32 threads)
 
 // ---- stable sort of (key, position); key = id, or vocab for a slot without a token (sorts behind every id) ------------------------
 // The dense form also has to zero every row of the table (the rows of the batch's tokens are overwritten by the sums): a write of the whole table, which
@@ -304,6 +305,9 @@ __global__ __launch_bounds__(1024) void embed_join_kernel(const unsigned* __rest
     }
 }
 
+// Tokens per call: every tile of a radix pass reads the counts of all tiles, so a pass grows with the square of the list (2^24 tokens: 8 192 tiles, 137 GB of counts
+// out of the caches).  Longer lists are added up over several calls with accumulate = 1.
+constexpr long EMBED_TOKENS = 1l << 24;
 // tokens per chunk
 static int embed_chunk(long n) { return n >= 32768 ? 32 : 16; }
 static size_t round256(size_t b) { return (b + 255) & ~(size_t)255; }
@@ -336,7 +340,8 @@ extern "C" int vitg_embed_lookup(const long long* ids, long n, const void* table
     const bool wide = D % 8 == 0 && ldt % 8 == 0 && ldo % 8 == 0 && aligned_to(table, 16) && aligned_to(out, 16);
     const int cv = D / (wide ? 8 : 4);
     const int tx = cv >= 512 ? 512 : (cv + 63) / 64 * 64, ty = tx >= 256 ? 1 : 256 / tx;
-    const dim3 grid((unsigned)((n + ty - 1) / ty)), block(tx, ty);
+    const long blocks = (n + ty - 1) / ty;
+    const dim3 grid((unsigned)(blocks < LOOKUP_BLOCKS ? blocks : LOOKUP_BLOCKS)), block(tx, ty);
     with_dtype(table_dtype, [&](auto ti) {
         typedef decltype(ti) TI;
         with_dtype(out_dtype, [&](auto to) {
@@ -350,14 +355,14 @@ extern "C" int vitg_embed_lookup(const long long* ids, long n, const void* table
 
 extern "C" int vitg_embed_backward_plan(long n, int D, long* workspace_bytes) {
     if (!workspace_bytes) return VITG_ERR_ARG;
-    if (n < 0 || n >= (1l << 31) || D <= 0) return VITG_ERR_SHAPE;
+    if (n < 0 || n > EMBED_TOKENS || D <= 0) return VITG_ERR_SHAPE;
     *workspace_bytes = n ? (long)embed_workspace(n, D).bytes : 0;
     return 0;
 }
 
 extern "C" int vitg_embed_backward(const long long* ids, long n, const void* dout, int dout_dtype, long ldd, long vocab, int D, float scale, void* dtable,
                                    int table_dtype, long ldt, int accumulate, void* workspace, long workspace_bytes, void* stream) {
-    if (n < 0 || vocab <= 0 || D <= 0 || n >= (1l << 31) || vocab >= (1l << 31) - 1 || ldt < D) return VITG_ERR_SHAPE;
+    if (n < 0 || vocab <= 0 || D <= 0 || n > EMBED_TOKENS || vocab >= (1l << 31) - 1 || ldt < D) return VITG_ERR_SHAPE;
     if (!dtable || (n && (!ids || !dout || !workspace))) return VITG_ERR_ARG;
     if (!dtype_ok(table_dtype) || !dtype_ok(dout_dtype)) return VITG_ERR_DTYPE;
     if (n && ldd < D) return VITG_ERR_SHAPE;

@@ -190,7 +190,7 @@ extern "C" int vitg_pool_score_save(const void* h, int h_dtype, long ldh, int fr
     if (frames <= 0) return 0;
     if (!h || !w || !b || !logits || !pooled) return VITG_ERR_ARG;
     if (!dtype_ok(h_dtype)) return VITG_ERR_DTYPE;
-    if (tokens_per_frame <= 0 || D <= 0 || ldh < D || ldp < D) return VITG_ERR_SHAPE;
+    if (tokens_per_frame <= 0 || D <= 0 || ldh < D || ldp < D || frames >= (1 << 22)) return VITG_ERR_SHAPE;      // (a launch has fewer than 2^32 threads)
     if (D % 4 || ldh % 4 || ldp % 4 || !aligned_to(h, 4 * dtype_size(h_dtype)) || !aligned_to(w, 16) || !aligned_to(pooled, 16)) return VITG_ERR_ALIGN;
     const bool wide = h_dtype != DT_F32 && D % 8 == 0 && ldh % 8 == 0 && aligned_to(h, 16);
     const int cv = D / (wide ? 8 : 4);
@@ -226,9 +226,9 @@ extern "C" int vitg_pool_score_backward(const float* pooled, long ldp, int frame
     if ((dh && lddh < D) || (dw && frames && ldp < D)) return VITG_ERR_SHAPE;
     if (D % 4 || !aligned_to(w, 16) || (dw && (ldp % 4 || !aligned_to(pooled, 16))) || (dh && (lddh % 4 || !aligned_to(dh, 4 * dtype_size(dh_dtype))))) return VITG_ERR_ALIGN;
     const int wblocks = dw ? ceil_div(D, 64) : db ? 1 : 0;
-    const long blocks = wblocks + (dh ? (long)frames * ceil_div(tokens_per_frame, DH_ROWS) : 0);
+    const long blocks = wblocks + (dh ? (long)frames * (((long)tokens_per_frame + DH_ROWS - 1) / DH_ROWS) : 0);
     if (!blocks) return 0;
-    if (blocks >= (1l << 31)) return VITG_ERR_SHAPE;
+    if (blocks >= (1l << 24)) return VITG_ERR_SHAPE;     // (a launch has fewer than 2^32 threads)
     const unsigned grid = (unsigned)blocks;
     const bool wide = dh && dh_dtype != DT_F32 && D % 8 == 0 && lddh % 8 == 0 && aligned_to(dh, 16);
     with_dtype(dh ? dh_dtype : (int)DT_F32, [&](auto ti) {
