@@ -37,16 +37,21 @@ constexpr long LOOKUP_BLOCKS = 1l << 20;                 // (a launch has fewer 
 // The dense form also has to zero every row of the table (the rows of the batch's tokens are overwritten by the sums): a write of the whole table, which
 // keeps HBM busy while the sort uses a few CUs.  So the zeroing rides along: each sort launch carries extra blocks behind its own that zero a share of the rows.
 struct ZeroRows { void* table; long pitch, bytes, begin, end; int blocks; };      // rows [begin, end), `bytes` of every `pitch`, by the last `blocks` of the grid
-__device__ __forceinline__ void zero_rows(const ZeroRows& z, int block) {
-    if ((z.pitch | z.bytes | (long)(uintptr_t)z.table) & 15) {
+// AROUND (the radix passes): non-temporal stores, which leave no dirty lines for the sums behind them to write back: 20 480 tokens of 3584 bf16 into 1 000 / 17 000 /
+// 152 064 rows take 70 / 92 / 266 us against 70 / 101 / 286, and with a pass that reads the table behind them 78 / 121 / 485 against 78 / 128 / 499.  The short
+// lists' single launch is over before HBM has taken that much, and the ordinary form wins there: 5 000 tokens, 17 000 rows 36 us against 42 (59 against 67 with the reader).
+template <bool AROUND> __device__ __forceinline__ void zero_rows(const ZeroRows& z, int block) {
+    auto run = [&](auto zero) {
+        typedef decltype(zero) Z;
         for (long r = z.begin + block; r < z.end; r += z.blocks)
-            for (long c = threadIdx.x * 8l; c < z.bytes; c += blockDim.x * 8l) *(u32x2*)((char*)z.table + r * z.pitch + c) = u32x2{0, 0};
-    } else {
-        for (long r = z.begin + block; r < z.end; r += z.blocks)
-            for (long c = threadIdx.x * 16l; c < z.bytes; c += blockDim.x * 16l) *(u32x4*)((char*)z.table + r * z.pitch + c) = u32x4{0, 0, 0, 0};
-    }
+            for (long c = threadIdx.x * (long)sizeof(Z); c < z.bytes; c += blockDim.x * (long)sizeof(Z)) {
+                Z* const p = (Z*)((char*)z.table + r * z.pitch + c);
+                if constexpr (AROUND) __builtin_nontemporal_store(zero, p); else *p = zero;
+            }
+    };
+    if ((z.pitch | z.bytes | (long)(uintptr_t)z.table) & 15) run(u32x2{0, 0}); else run(u32x4{0, 0, 0, 0});
 }
-__global__ __launch_bounds__(256) void zero_rows_kernel(const ZeroRows z) { zero_rows(z, blockIdx.x); }
+__global__ __launch_bounds__(256) void zero_rows_kernel(const ZeroRows z) { zero_rows<true>(z, blockIdx.x); }
 
 constexpr int SORT_BITS = 9, SORT_BINS = 1 << SORT_BITS, SORT_TILE = 2048, SORT_THREADS = 256;
 
@@ -58,7 +63,7 @@ constexpr int RANK_MAX = 15360, RANK_WAVES = 16;         // 60 KiB of keys
 __global__ __launch_bounds__(RANK_WAVES * 64) void sort_rank_kernel(const long long* __restrict__ ids, int n, unsigned vocab, unsigned* __restrict__ key_out,
                                                                     unsigned* __restrict__ pos_out, int blocks, const ZeroRows z) {
     extern __shared__ __attribute__((aligned(16))) unsigned keys[];      // n keys, padded to a multiple of 16 with the largest value
-    if ((int)blockIdx.x >= blocks) { zero_rows(z, (int)blockIdx.x - blocks); return; }
+    if ((int)blockIdx.x >= blocks) { zero_rows<false>(z, (int)blockIdx.x - blocks); return; }
     __shared__ unsigned part[64];
     const int padded = (n + 15) & ~15;
 #pragma unroll 4
@@ -96,7 +101,7 @@ __global__ __launch_bounds__(RANK_WAVES * 64) void sort_rank_kernel(const long l
 template <bool FIRST>
 __global__ __launch_bounds__(SORT_THREADS) void sort_count_kernel(const long long* __restrict__ ids, const unsigned* __restrict__ key_in, long n, unsigned vocab,
                                                                   int shift, unsigned* __restrict__ counts, int tiles, const ZeroRows z) {
-    if ((int)blockIdx.x >= tiles) { zero_rows(z, (int)blockIdx.x - tiles); return; }
+    if ((int)blockIdx.x >= tiles) { zero_rows<true>(z, (int)blockIdx.x - tiles); return; }
     __shared__ unsigned bins[SORT_BINS];
     for (int b = threadIdx.x; b < SORT_BINS; b += SORT_THREADS) bins[b] = 0;
     __syncthreads();
@@ -114,7 +119,7 @@ __global__ __launch_bounds__(SORT_THREADS) void sort_scatter_kernel(const long l
                                                                     const unsigned* __restrict__ pos_in, long n, unsigned vocab, int shift, int tiles,
                                                                     const unsigned* __restrict__ counts, unsigned* __restrict__ key_out, unsigned* __restrict__ pos_out,
                                                                     const ZeroRows z) {
-    if ((int)blockIdx.x >= tiles) { zero_rows(z, (int)blockIdx.x - tiles); return; }
+    if ((int)blockIdx.x >= tiles) { zero_rows<true>(z, (int)blockIdx.x - tiles); return; }
     constexpr int WAVES = SORT_THREADS / 64, ROUNDS = SORT_TILE / SORT_THREADS, BPT = SORT_BINS / SORT_THREADS;
     __shared__ unsigned next[WAVES][SORT_BINS];          // next free slot of a digit for one wave's keys
     __shared__ unsigned wave_total[WAVES];
