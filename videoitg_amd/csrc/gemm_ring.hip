@@ -5,6 +5,8 @@
 //   step t:  wait until this wave's DMA of tile t+1 has landed (three newer tiles stay in flight) and its fragment reads of tile t are done; barrier;
 //            DMA of tile t+4 into the slot of tile t (every wave holds tile t in registers); fragment reads of tile t+1; the 32 MFMAs of tile t.
 // Four waves as 2 x 2, 64 x 64 each, v_mfma_f32_16x16x32, MFMA "A" = weight rows (a lane holds 4 consecutive output features of one row).
+// Measured: a step takes 0.35 us with one block on the chip (the barrier and the LDS reads), 0.7 us with a block on every CU (L2); K = 1024, N = 4096, 512 rows with
+// the SwiGLU epilogue 12 us = 358 TFLOP/s, against 16 on the 128x128 tile of gemm.hip and 23 on the 256x256 one.
 // LDS images and the XOR swizzles are those of gemm_mi16.hip (128-B rows, 16-B chunk ^ ((row >> 1) & 7); K-major weights: 256-B rows, 32-B chunk ^
 // (((row >> 3) & 1) * 4 + (row & 3)), read with ds_read_b64_tr_b16).
 #include "gemm_common.h"

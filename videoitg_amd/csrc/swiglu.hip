@@ -8,6 +8,10 @@
 // Backward: dX runs on the GEMM form that takes W as it lies (contraction along W's rows); dW's contraction runs along the rows of both operands, so dGU comes
 // out of its elementwise kernel in both orders and X passes through a tile transpose in front of the ordinary NT GEMM.  dGU is rounded to the 16-bit type once -
 // the matrix pipe's operand type - and every sum over it is fp32.
+//
+// Measured at 3584 x 37888 (bf16; large library products of these shapes run at 1 307 - 1 436 TFLOP/s): one row 49 us = 5.6 TB/s of W; 12 860 rows with
+// pre-activations 2.67 ms = 1 309 TFLOP/s; their backward 5.73 ms: 0.80 in front (4.1 GB, 5.2 TB/s), dX and dW 2.46 each = 1 420 TFLOP/s; 1 607 rows (fp16)
+// 0.88 ms: 0.08 + dX 0.43 (two shares, K-major) + dW 0.38 + the join 0.01.
 #include "train_common.h"
 #include "gemm_common.h"
 

@@ -6,7 +6,11 @@
 // Two passes over the data, each bound by HBM.  Pass 1: a fixed grid walks the 64 KiB pieces of up to 96 tensors (their addresses ride in the kernel
 // arguments: nothing is uploaded, so a call can be captured into a graph) and leaves one sum per block; pass 2: every block adds the sums in the same
 // order, so all blocks hold the same factor, and scales its pieces.  Squares are summed in fp64: the square of any fp32 / bf16 value is representable
-// there, so neither large nor tiny gradients change the norm, and the fixed order gives the same bits on every call.
+// there, so neither large nor tiny gradients change the norm, and the fixed order gives the same bits on every call.  Pass 2 walks the pieces from the end: it
+// begins with what pass 1 has left in the last-level cache.
+//
+// Measured: four decoder layers (1.86 GB, bf16 matrices and fp32 vectors): sums 299 us = 6.2 TB/s, scaling 716 us = 5.2 TB/s (a copy: 5.1);
+// six tensors of a projector and a head (fp32, 68 MB): 14 + 24 us, mostly launch and the walk's tail.
 #include "train_common.h"
 #include <math.h>
 #include <stdlib.h>

@@ -6,9 +6,6 @@
 
 namespace vitg {
 
-template <typename T> __device__ __forceinline__ float to_f32(T v) { return (float)v; }
-template <typename T> __device__ __forceinline__ T from_f32(float v) { return (T)v; }       // round to nearest even (a plain copy for fp32)
-
 // V consecutive elements of type T <-> fp32 values; p aligned to the vector
 template <typename T, int V> struct Pack { typedef T type __attribute__((ext_vector_type(V))); };
 template <typename T, int V> __device__ __forceinline__ void load_vec(const T* p, float (&v)[V]) {

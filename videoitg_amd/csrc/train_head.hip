@@ -7,6 +7,9 @@
 //
 // The backward of the mean needs no second look at h: the forward keeps the frame means (frames x D fp32, 1 / tokens of h), so a step reads h once and
 // writes dh once - HBM-bound on both sides.
+//
+// Measured at D = 3584: 512 frames x 25 tokens, fp32 (184 MB): means and scores 32 us = 5.7 TB/s, gradients 29 us = 6.3 TB/s; 61 frames x 256 tokens, bf16
+// (112 MB): means 18 us = 6.3 TB/s + scores 3 us, gradients 19 us = 5.9 TB/s; the loss 3 - 4 us, a launch.
 #include "train_common.h"
 
 namespace vitg {
@@ -51,7 +54,7 @@ __global__ __launch_bounds__(1024) void pool_score_save_kernel(const T* __restri
     }
 }
 
-// fewer frames than CUs: a block takes 64 column groups of one frame, its four waves a quarter of the rows each (joined in order); pool_dot_kernel takes the
+// few, long frames: a block takes 64 column groups of one frame, its four waves a quarter of the rows each (joined in order); pool_dot_kernel takes the
 // scores from the means
 template <typename T, int V, bool AROUND>
 __global__ __launch_bounds__(256) void pool_mean_kernel(const T* __restrict__ h, long ldh, int tokens, int cv, float* __restrict__ pooled, long ldp) {
@@ -194,7 +197,10 @@ extern "C" int vitg_pool_score_save(const void* h, int h_dtype, long ldh, int fr
     if (D % 4 || ldh % 4 || ldp % 4 || !aligned_to(h, 4 * dtype_size(h_dtype)) || !aligned_to(w, 16) || !aligned_to(pooled, 16)) return VITG_ERR_ALIGN;
     const bool wide = h_dtype != DT_F32 && D % 8 == 0 && ldh % 8 == 0 && aligned_to(h, 16);
     const int cv = D / (wide ? 8 : 4);
-    const bool few = frames < device_cu_count(current_device()) && tokens_per_frame >= 8 && cv > 64;
+    // One block per frame, or the rows of a frame over several blocks and a second launch for the scores: the second form where a frame is long and the frames'
+    // waves (64 column groups each) are fewer than five a CU.  bf16, D = 3584, us: 8 x 196 14.6 against 11.0, 61 x 256 28.5 against 20.7, 128 x 196 34.6 against
+    // 31.4; but 61 x 64 7.8 against 10.6 (the launch), 200 x 256 55 against 59, 512 x 256 143 against 152.  D = 1024: 160 x 196 20.9 against 13.8
+    const bool few = (long)frames * cv < device_cu_count(current_device()) * 5l * 64 && tokens_per_frame >= 128 && cv > 64;
     const int threads = cv >= 1024 ? 1024 : (cv + 63) / 64 * 64;
     hipStream_t s = (hipStream_t)stream;
     with_dtype(h_dtype, [&](auto ti) {
