@@ -559,6 +559,41 @@ def test_given_workspaces_of_exactly_the_planned_size(ops):
 
 
 @pytest.mark.gpu
+def test_nan_and_infinity_stay_where_they_belong(ops):
+    nan = float("nan")
+    for n in (40, 20000):                                # rank sort, radix passes
+        ids = torch.randint(0, 50, (n,), generator=torch.Generator().manual_seed(n)).cuda()
+        ids[::3] = -200
+        ids[1::7] = 50
+        out = ids < 0
+        out |= ids >= 50
+        dout = torch.ones(n, 8, device="cuda")
+        dout[out] = nan
+        got = ops.embed_backward(ids, dout, torch.empty(50, 8, device="cuda"))
+        assert torch.equal(got[:, 0].cpu(), torch.bincount(ids[~out], minlength=50).float().cpu())
+        table = torch.full((50, 8), nan, device="cuda")
+        table[:49] = 2.0
+        rows = ops.embed_lookup(ids, table, torch.empty(n, 8, device="cuda"))
+        assert (rows[out] == 0).all() and torch.equal(rows.isnan().any(1), ids == 49)
+    for m, n, k in ((9, 128, 64), (100, 256, 192), (300, 32768, 64), (600, 1024, 128)):
+        x, w, dout = randn(m, k, dtype=BF16).cuda(), randn(n, k, dtype=BF16, seed=1).cuda(), randn(m, n // 2, dtype=BF16, seed=2).cuda()
+        x[m // 2], x[m - 1] = nan, float("inf")
+        bad = torch.zeros(m, dtype=torch.bool, device="cuda")
+        bad[m // 2] = bad[m - 1] = True
+        act, gu, dx = torch.empty(m, n // 2, dtype=BF16, device="cuda"), torch.empty(m, n, dtype=BF16, device="cuda"), torch.empty_like(x)
+        ops.swiglu(x, w, act, gu=gu)
+        assert act[~bad].isfinite().all() and gu[~bad].isfinite().all() and not act[m // 2].isfinite().any()
+        ops.swiglu_backward(dout, gu, x, w, dx=dx)
+        assert dx[~bad].isfinite().all() and not dx[m // 2].isfinite().any()
+    for frames, tokens in ((5, 7), (5, 200)):
+        h = torch.ones(frames * tokens, 1024, device="cuda")
+        h[2 * tokens + tokens // 2] = nan
+        z, pooled = torch.empty(frames, device="cuda"), torch.empty(frames, 1024, device="cuda")
+        ops.pool_score_save(h, frames, tokens, 1024, torch.ones(1024, device="cuda"), torch.zeros(1, device="cuda"), z, pooled)
+        assert z.isnan().tolist() == [False, False, True, False, False] and (pooled[[0, 1, 3, 4]] - 1).abs().max() <= tokens * U32
+
+
+@pytest.mark.gpu
 def test_calls_on_two_streams_at_once(ops):
     """the same operators on other data on two streams, without a wait in between: each result is its own"""
     from videoitg_amd.torch_ops import K
