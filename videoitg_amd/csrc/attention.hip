@@ -266,8 +266,7 @@ __global__ __launch_bounds__(NW * 64, (NW == 8 && D == 72 && DMA) ? 4 : 2) void 
                 for (int r = 0; r < 16; ++r) o[i][r] *= alpha;
             m_run = m_new;
         }
-        // The softmax block is VALU-issue bound (PMC: VALU busy > MFMA busy), so the exponent arguments and the row sum
-        // use packed fp32 (v_pk_fma_f32 / v_pk_add_f32: two scores per issue); the 32 v_exp_f32 stay scalar.
+        // The softmax block is VALU-issue bound (PMC: VALU busy > MFMA busy): one FMA, one v_exp_f32 and one add per score, in two chains of sums.
         f32x2 psum2 = {0.f, 0.f};
         const f32x2 sc2 = {a.scale_log2e, a.scale_log2e};
         const f32x2 nm2 = {-m_run, -m_run};
@@ -426,10 +425,7 @@ __global__ __launch_bounds__(NW * 64, (NW == 8 && D == 72 && DMA) ? 4 : 2) void 
             for (int g4 = 0; g4 < 4; ++g4) {
                 const int d = dt * 32 + 8 * g4 + 4 * h;
                 if (d < D) {
-                    typename T16<T>::vec4 w;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) w[e] = T16<T>::from_f32(o[dt][g4 * 4 + e] * inv);
-                    *(typename T16<T>::vec4*)(op + d) = w;
+                    *(typename T16<T>::vec4*)(op + d) = attn_out4<T>(o[dt][g4 * 4 + 0], o[dt][g4 * 4 + 1], o[dt][g4 * 4 + 2], o[dt][g4 * 4 + 3], inv);
                 }
             }
     }

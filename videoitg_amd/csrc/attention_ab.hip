@@ -39,7 +39,7 @@ constexpr float AB_LAZY_RESCALE_LOG2 = 8.0f;      // see attention_sp.hip: runni
 // QS (scores leave the matrix pipe ready for exp2; needs Q pre-multiplied by scale * log2(e) - vitg_attention variant bit 1 - which the engine folds
 // into the q rows of the tower's qkv weights): the same pad column on the QK^T side.  K's pad chunk (d 72..79) holds [1, 0, ..], Q's pad element 72
 // holds -shift of its query, so S' = K Q'^T - shift comes out of the MFMAs that run anyway and P = exp2(S') needs neither the scale multiply nor
-// the max subtraction (one packed FMA per score pair less).  Softmax is shift-invariant per query, so the shift only has to be CONSISTENT between
+// the max subtraction (one FMA per score less).  Softmax is shift-invariant per query, so the shift only has to be CONSISTENT between
 // the numerator, the row sum (same P) and the accumulator rescale (alpha = exp2(old shift - new shift)): it is the running max rounded to 16 bits,
 // moved - as before - only when a tile's scores exceed it by more than 2^8, and then that one tile subtracts the step on the VALU.
 // NKT_C (round 6: "a compile-time S = 1024 specialisation with no tail / key-count path for the R = 448 tower"): > 0 = the number of
@@ -436,10 +436,7 @@ __global__ __launch_bounds__(NW * 64, 4) void attn_ab_kernel(AttnArgs a) {
                 for (int dt = 0; dt < DT; ++dt) {
                     const int d = dt * 16 + 4 * g16;
                     if (d < D) {
-                        typename T16<T>::vec4 w;
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) w[e] = T16<T>::from_f32(o16[dt][qt][e] * iq);
-                        *(typename T16<T>::vec4*)(op + d) = w;
+                        *(typename T16<T>::vec4*)(op + d) = attn_out4<T>(o16[dt][qt][0], o16[dt][qt][1], o16[dt][qt][2], o16[dt][qt][3], iq);
                     }
                 }
             }
@@ -454,10 +451,7 @@ __global__ __launch_bounds__(NW * 64, 4) void attn_ab_kernel(AttnArgs a) {
             for (int g4 = 0; g4 < 4; ++g4) {
                 const int d = dt * 32 + 8 * g4 + 4 * h;
                 if (d < D) {
-                    typename T16<T>::vec4 w;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) w[e] = T16<T>::from_f32(o[dt][g4 * 4 + e] * inv);
-                    *(typename T16<T>::vec4*)(op + d) = w;
+                    *(typename T16<T>::vec4*)(op + d) = attn_out4<T>(o[dt][g4 * 4 + 0], o[dt][g4 * 4 + 1], o[dt][g4 * 4 + 2], o[dt][g4 * 4 + 3], inv);
                 }
             }
     }

@@ -435,10 +435,7 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_sp_kernel(AttnArgs a) {
                 T* op = (T*)a.o + b * a.o_bs + (long)head * a.o_hs + (long)qrow * a.o_rs;
 #pragma unroll
                 for (int dt = 0; dt < DT; ++dt) {
-                    typename T16<T>::vec4 w;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) w[e] = T16<T>::from_f32(o16[dt][qt][e] * iq);
-                    *(typename T16<T>::vec4*)(op + dt * 16 + 4 * g16) = w;
+                    *(typename T16<T>::vec4*)(op + dt * 16 + 4 * g16) = attn_out4<T>(o16[dt][qt][0], o16[dt][qt][1], o16[dt][qt][2], o16[dt][qt][3], iq);
                 }
             }
         }
@@ -452,10 +449,7 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_sp_kernel(AttnArgs a) {
             for (int g4 = 0; g4 < 4; ++g4) {
                 const int d = dt * 32 + 8 * g4 + 4 * h;
                 if (d < D) {
-                    typename T16<T>::vec4 w;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) w[e] = T16<T>::from_f32(o[dt][g4 * 4 + e] * inv);
-                    *(typename T16<T>::vec4*)(op + d) = w;
+                    *(typename T16<T>::vec4*)(op + d) = attn_out4<T>(o[dt][g4 * 4 + 0], o[dt][g4 * 4 + 1], o[dt][g4 * 4 + 2], o[dt][g4 * 4 + 3], inv);
                 }
             }
     }

@@ -1,5 +1,6 @@
 // Declarations shared by the attention kernels (attention.hip: per-tile loop; attention_sp.hip: software-pipelined loop).
 #pragma once
+#include <type_traits>
 #include "common.h"
 
 namespace vitg {
@@ -63,6 +64,24 @@ __device__ __forceinline__ void lds_dma_drain() {
 #if VITG_ASM_DMA
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 #endif
+}
+
+// Four neighbouring outputs of a query, o * inv, in 16 bits.  fp16: elements 0 and 3 in ONE rounding (v_fma_mixlo_f16), 1 and 2 rounded to fp32 first - the two
+// differ in one value of about 2^14, and the full-size fixtures hold this form bit for bit.  The empty asm keeps a lone conversion apart from its neighbours.
+template <typename T> __device__ __forceinline__ typename T16<T>::vec4 attn_out4(float o0, float o1, float o2, float o3, float inv) {
+    typename T16<T>::vec4 w;
+    if constexpr (std::is_same<T, f16_t>::value) {
+        f16_t w0 = (f16_t)(o0 * inv), w3 = (f16_t)(o3 * inv);
+        asm("" : "+v"(w0));
+        asm("" : "+v"(w3));
+        const f32x2 r = {mul_rounded(o1, inv), mul_rounded(o2, inv)};
+        typedef f16_t f16x2 __attribute__((ext_vector_type(2)));
+        const f16x2 m = __builtin_convertvector(r, f16x2);
+        w[0] = w0; w[1] = m[0]; w[2] = m[1]; w[3] = w3;
+    } else {
+        w[0] = T16<T>::from_f32(o0 * inv); w[1] = T16<T>::from_f32(o1 * inv); w[2] = T16<T>::from_f32(o2 * inv); w[3] = T16<T>::from_f32(o3 * inv);
+    }
+    return w;
 }
 
 constexpr int ATT_BK = 64;

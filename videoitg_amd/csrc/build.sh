@@ -4,11 +4,8 @@
 #   build.sh --profiling [extra hipcc flags]   libvideoitg_hip_prof.so: + research GEMM variants and ablation switches
 #                                              (include/videoitg_hip_profiling.h); loaded by tools/ only, never by the product
 set -euo pipefail
-# no packed fp32 forms (v_pk_add / mul / fma_f32) from hipcc: some of their forms have given wrong results on gfx950 now and then.  Without them hipcc contracts
-# products and sums at other places, so the sources named in PACKED - the forward's attention, norm, quantiser and split-precision kernels and the research GEMMs - are
-# compiled as they always were: their results are pinned bit for bit (tests/test_fullsize_parity.py's heavy-tailed video moves past its bound otherwise).
+# no packed fp32 forms (v_pk_add / mul / fma_f32) from hipcc: some of their forms have given wrong results on gfx950 now and then
 NOPK="-Xclang -target-feature -Xclang -packed-fp32-ops"
-PACKED=" attention attention_sp attention_ab attention_w4 elementwise split gemm_fp8 gemm_w4 gemm_wf gemm_pe "
 HERE="$(cd "$(dirname "${BASH_SOURCE[0]}")" && pwd)"
 HIPCC="${HIPCC:-/opt/rocm/bin/hipcc}"
 SRCS="device gemm gemm256 gemm_mi16 gemm_fp8 attention attention_sp attention_ab elementwise preprocess probe split train_embed train_clip train_head swiglu gemm_ring"
@@ -40,11 +37,10 @@ for f in $SRCS; do
   src="$HERE/$f.hip"; obj="$OBJ/$f.o"
   [ -f "$src" ] || continue
   objs+=("$obj")
-  if [ ! -f "$obj" ] || [ "$src" -nt "$obj" ] || [ "$HERE/common.h" -nt "$obj" ] || [ "$HERE/gemm_common.h" -nt "$obj" ] || [ "$HERE/attn_common.h" -nt "$obj" ] || [ "$HERE/train_common.h" -nt "$obj" ] || [ "$HERE/../../include/videoitg_hip.h" -nt "$obj" ]; then
-    extra="$NOPK"
-    case "$PACKED" in *" $f "*) extra="" ;; esac
-    [ "$f" = "attention_w4" ] && extra="$extra -fno-slp-vectorize"      # its VALU stream is hand-placed in single-issue forms (see st_scale in the file)
-    "$HIPCC" --offload-arch=gfx950 -O3 -std=c++17 -fPIC $DEFS $extra -c "$src" -o "$obj" "$@" &
+  if [ ! -f "$obj" ] || [ "$src" -nt "$obj" ] || [ "$HERE/build.sh" -nt "$obj" ] || [ "$HERE/common.h" -nt "$obj" ] || [ "$HERE/gemm_common.h" -nt "$obj" ] || [ "$HERE/attn_common.h" -nt "$obj" ] || [ "$HERE/train_common.h" -nt "$obj" ] || [ "$HERE/../../include/videoitg_hip.h" -nt "$obj" ]; then
+    extra=""
+    [ "$f" = "attention_w4" ] && extra="-fno-slp-vectorize"      # its VALU stream is hand-placed in single-issue forms (see st_scale in the file)
+    "$HIPCC" --offload-arch=gfx950 -O3 -std=c++17 -fPIC $NOPK $DEFS $extra -c "$src" -o "$obj" "$@" &
     pids+=($!)
     compiled="$compiled $f"
   else

@@ -20,6 +20,7 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x8 __attribute__((ext_vector_type(8)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
@@ -58,6 +59,13 @@ template <typename V, typename U> __device__ __forceinline__ V bitcast(const U& 
     return __builtin_bit_cast(V, u);
 }
 
+// a * b rounded to fp32 by itself: without the pragma hipcc contracts the product into the sum that uses it, or not, by how it has vectorised the loop - and a
+// result that is pinned (the norms' variance, the score's dot product) would move with the compiler's flags
+__device__ __forceinline__ float mul_rounded(float a, float b) {
+#pragma clang fp contract(off)
+    return a * b;
+}
+
 // ---- wave / block reductions -------------------------------------------------------------------
 __device__ __forceinline__ float wave_sum(float v) {
 #pragma unroll
@@ -79,10 +87,9 @@ __device__ __forceinline__ float gelu_tanh_f(float x) {
     const float a = x * __builtin_fmaf(x * x, -0.10294324302f, -2.30220819814f);
     return x * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(a));
 }
-// two values at a time on the packed fp32 VALU forms (v_pk_mul_f32 / v_pk_fma_f32 / v_pk_add_f32) - the same operations in the same order as the
-// scalar forms, so the results are bit-identical.  (Half the instructions, NOT half the time: tools/ubench/valu_rate.hip measures 5.4 clocks per
-// v_pk_fma_f32 against 2.7 per v_fma_f32 on gfx950 - the same rate per value.  The gain of the epilogue rewrite came from taking the tests out of
-// the quad loop, profiles/r03_gemm_epilogue.md.)
+// two values at a time - the same operations in the same order as the scalar forms, so the results are bit-identical.  (csrc/build.sh compiles without the packed
+// fp32 instructions; nothing is lost by that: tools/ubench/valu_rate.hip measures 5.4 clocks per v_pk_fma_f32 against 2.7 per v_fma_f32 on gfx950, the
+// same rate per value.  The gain of the epilogue rewrite came from taking the tests out of the quad loop, profiles/r03_gemm_epilogue.md.)
 __device__ __forceinline__ f32x2 gelu_tanh_f2(f32x2 x) {
     const f32x2 ca = {-0.10294324302f, -0.10294324302f}, cb = {-2.30220819814f, -2.30220819814f}, one = {1.0f, 1.0f};
     const f32x2 a = x * __builtin_elementwise_fma(x * x, ca, cb);

@@ -132,7 +132,7 @@ __global__ void norm_kernel(const float* __restrict__ x, int ldx, const float* _
                 const int c = (i * 64 + lane) * 4;
                 if (c < D) {
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) { const float d = v[i][e] - mean; q += d * d; }
+                    for (int e = 0; e < 4; ++e) { const float d = v[i][e] - mean; q += mul_rounded(d, d); }
                 }
             }
             q = wave_sum(q);
@@ -201,7 +201,7 @@ __global__ void ln16_kernel(const T* __restrict__ x, int ldx, const float* __res
             const int c = (i * 64 + lane) * 8;
             if (c < D) {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) { const float d = f[i][e] - mean; q += d * d; }
+                for (int e = 0; e < 8; ++e) { const float d = f[i][e] - mean; q += mul_rounded(d, d); }
             }
         }
         q = wave_sum(q);
@@ -214,11 +214,13 @@ __global__ void ln16_kernel(const T* __restrict__ x, int ldx, const float* __res
             if (c < D) {
                 const f32x4 w0 = *(const f32x4*)(w + c), w1 = *(const f32x4*)(w + c + 4);
                 const f32x4 b0 = *(const f32x4*)(bia + c), b1 = *(const f32x4*)(bia + c + 4);
+                f32x8 r;                                     // fp32 first, then the 16-bit rounding: as one vector the pair is not folded into v_fma_mix (one rounding)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    o[e] = T16<T>::from_f32((f[i][e] - mean) * rstd * w0[e] + b0[e]);
-                    o[e + 4] = T16<T>::from_f32((f[i][e + 4] - mean) * rstd * w1[e] + b1[e]);
+                    r[e] = (f[i][e] - mean) * rstd * w0[e] + b0[e];
+                    r[e + 4] = (f[i][e + 4] - mean) * rstd * w1[e] + b1[e];
                 }
+                o = __builtin_convertvector(r, vec8);
             }
             *(vec8*)(out + row * ldo + c) = o;
         }
@@ -267,12 +269,12 @@ __global__ __launch_bounds__(256) void ln16r4_kernel(const T* __restrict__ x, in
         for (int i = 0; i < NC; ++i)
 #pragma unroll
             for (int e = 0; e < 8; ++e) s += T16<T>::to_f32(v[i][e]);
-        const float mean = row16_sum(s) * invD;
+        const float mean = mul_rounded(row16_sum(s), invD);
         float qq = 0.f;
 #pragma unroll
         for (int i = 0; i < NC; ++i)
 #pragma unroll
-            for (int e = 0; e < 8; ++e) { const float d = T16<T>::to_f32(v[i][e]) - mean; qq += d * d; }
+            for (int e = 0; e < 8; ++e) { const float d = T16<T>::to_f32(v[i][e]) - mean; qq += mul_rounded(d, d); }
         const float rstd = rsqrtf(row16_sum(qq) * invD + eps);
         const long row = q * 4 + rsel;
         if (row < M) {
@@ -282,13 +284,13 @@ __global__ __launch_bounds__(256) void ln16r4_kernel(const T* __restrict__ x, in
                 const int c = i * 128 + sub * 8;
                 const f32x4 w0 = *(const f32x4*)(w + c), w1 = *(const f32x4*)(w + c + 4);
                 const f32x4 b0 = *(const f32x4*)(bia + c), b1 = *(const f32x4*)(bia + c + 4);
-                vec8 o;
+                f32x8 r;                                     // (as in ln16_kernel)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    o[e] = T16<T>::from_f32((T16<T>::to_f32(v[i][e]) - mean) * rstd * w0[e] + b0[e]);
-                    o[e + 4] = T16<T>::from_f32((T16<T>::to_f32(v[i][e + 4]) - mean) * rstd * w1[e] + b1[e]);
+                    r[e] = (T16<T>::to_f32(v[i][e]) - mean) * rstd * w0[e] + b0[e];
+                    r[e + 4] = (T16<T>::to_f32(v[i][e + 4]) - mean) * rstd * w1[e] + b1[e];
                 }
-                *(vec8*)(orow + i * 128) = o;
+                *(vec8*)(orow + i * 128) = __builtin_convertvector(r, vec8);
             }
             for (int c = D + sub * 8; c < ldo; c += 128) *(vec8*)(out + row * ldo + c) = vec8{};
         }
@@ -319,15 +321,15 @@ __global__ void rope_kernel(T* __restrict__ qkv, int ld, const float* __restrict
     typedef typename T16<T>::vec4 v4;
     v4 a = *(v4*)p, b = *(v4*)(p + half);
     const f32x4 c = *(const f32x4*)(cs + n * half + j * 4), s = *(const f32x4*)(sn + n * half + j * 4);
-    v4 ra, rb;
+    f32x4 ra, rb;                                        // (fp32 first, then the 16-bit rounding, as in ln16_kernel)
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
         const float x1 = T16<T>::to_f32(a[e]), x2 = T16<T>::to_f32(b[e]);
-        ra[e] = T16<T>::from_f32(x1 * c[e] - x2 * s[e]);
-        rb[e] = T16<T>::from_f32(x2 * c[e] + x1 * s[e]);
+        ra[e] = x1 * c[e] - x2 * s[e];
+        rb[e] = x2 * c[e] + x1 * s[e];
     }
-    *(v4*)p = ra;
-    *(v4*)(p + half) = rb;
+    *(v4*)p = __builtin_convertvector(ra, v4);
+    *(v4*)(p + half) = __builtin_convertvector(rb, v4);
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -443,7 +445,7 @@ __global__ void pool_score_kernel(const float* __restrict__ h, int ldh, int tok,
         f32x4 s = {0.f, 0.f, 0.f, 0.f};
         for (int j = 0; j < tok; ++j) s += *(const f32x4*)(base + (long)j * ldh + c);
         const f32x4 ww = *(const f32x4*)(w + c);
-        acc += s[0] * ww[0] + s[1] * ww[1] + s[2] * ww[2] + s[3] * ww[3];
+        acc += mul_rounded(s[0], ww[0]) + mul_rounded(s[1], ww[1]) + mul_rounded(s[2], ww[2]) + mul_rounded(s[3], ww[3]);
     }
     acc = wave_sum(acc);
     if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = acc;

@@ -494,7 +494,7 @@ __global__ __launch_bounds__(256) void norm_quant_kernel(const TI* __restrict__ 
             const int c = (i * 64 + lane) * 4;
             if (c < D) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) { const float d = v[i][e] - mean; q += d * d; }
+                for (int e = 0; e < 4; ++e) { const float d = v[i][e] - mean; q += mul_rounded(d, d); }
             }
         }
         rstd = rsqrtf(wave_sum(q) / D + eps);

@@ -56,7 +56,7 @@ __global__ __launch_bounds__(256) void norm_split_kernel(const float* __restrict
             const int c = (i * 64 + lane) * 4;
             if (c < D) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) { const float d = v[i][e] - mean; q += d * d; }
+                for (int e = 0; e < 4; ++e) { const float d = v[i][e] - mean; q += mul_rounded(d, d); }
             }
         }
         q = wave_sum(q);
