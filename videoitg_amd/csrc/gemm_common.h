@@ -41,6 +41,8 @@ struct GemmArgs {
     unsigned* xcd_sync;       // profiling build, gemm_flags bit26: 8 per-XCD arrival counters (128 B apart), zeroed before the launch
     int sk_units, sk_kt;      // stream-K (vitg_gemm_streamk, gemm_mi16.hip): K-tile units per block / K-tiles per output tile; 0 = off
     void* gu; int ldgu;       // MODE_SWIGLU, SAVE form (vitg_swiglu): the 16-bit pre-activations [gate 32 | up 32]... for the backward pass, [M, N]
+    int res_last;             // MODE_F32 on the tiles of gemm_mi16.hip: the residual is added once, in the epilogue, instead of starting the accumulators (a residual
+                              // far larger than the product - a gradient over many batches - would round the sum at its own magnitude in every K-step)
     int split_k;              // MODE_F32 only: gridDim.y = split_k blocks share one output tile, block y accumulates its K range and
     long split_stride;        // writes the raw fp32 partial tile to out + y * split_stride floats (vitg_gemm_splitk reduces them)
     // patch embedding with the im2col inside the A-tile loader (vitg_patch_embed16; gemm_mi16.hip PATCH instantiations): A = pixel_values

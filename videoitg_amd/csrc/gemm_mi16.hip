@@ -186,7 +186,7 @@ __global__ __launch_bounds__(G16_THREADS, 2) void gemm16_kernel(GemmArgs g_) {
     // Accumulators: zero, or - fp32 residual update without activation - the residual tile itself (the read half of the
     // read-modify-write then overlaps the main loop; these loads are older than every DMA in the vmcnt queue)
     // (MODE_RES16 = vitg_gemm_res16: the 16-bit residual stream of the tower, or the fp32 position table, into a 16-bit output)
-    const bool acc_from_res = (MODE == MODE_F32 && g.res != nullptr && g.act == VITG_ACT_NONE) || RES16;
+    const bool acc_from_res = (MODE == MODE_F32 && g.res != nullptr && g.act == VITG_ACT_NONE && !g.res_last) || RES16;
     // 16-bit output with a bias and no residual: the accumulators START at the bias (a lane's four features are the same for all its row tiles), so
     // the epilogue has no add - the initialisation costs the same moves as zeroing.  gemm_flags bit27 keeps the add in the epilogue (A/B)
     const bool bias_init = MODE == MODE_STORE16 && g.bias != nullptr && !(g.flags & 0x8000000);
