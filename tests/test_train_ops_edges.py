@@ -35,3 +35,40 @@ def test_weight_gradient_is_added_once_on_every_route(ops, dtype, m, k, n):
         dw = old.clone()
         ops.swiglu_backward(dout, gu, x, w, dx=dx, dw=dw, accumulate=True)
         assert torch.equal(dw, want), f"{int((dw != want).sum())} of {dw.numel()} rounded more than once"
+
+
+@pytest.mark.gpu
+def test_loss_of_the_most_logits_a_call_takes(ops):
+    """2^31 - 1 logits and frames: an index that wraps behind the last one reads and writes outside.  All logits 0 but the last few, so that everything is known"""
+    n = (1 << 31) - 1
+    z, y = torch.zeros(n, device="cuda"), torch.zeros(n, device="cuda")
+    z[-3:] = torch.tensor([40.0, -40.0, 2.0], device="cuda")
+    y[:1 << 30] = 1.0                                    # one label more than none of them: pos_weight = sqrt((2^30 - 1) / 2^30), 1 in fp32
+    loss, weight, dz = ops.bce_loss_backward(z, y, scale=float(1 << 31))
+    assert weight.item() == 1.0
+    assert abs(loss.item() / 0.6931471805599453 - 1) <= 2.0 ** -20
+    assert (dz[:1 << 30] == -0.5).all() and (dz[1 << 30:-3] == 0.5).all()
+    want = torch.sigmoid(torch.tensor([40.0, -40.0, 2.0], dtype=torch.float64))
+    assert ((dz[-3:].double().cpu() - want).abs() <= want * 2.0 ** -20).all()
+    plain, weight = ops.bce_loss(z, y)
+    assert weight.item() == 1.0 and 0.5 < plain.item() < 0.9      # (2^21 fp32 terms a thread, rounded at up to 2^21)
+    db = torch.zeros(1, device="cuda")
+    ops.pool_score_backward(torch.empty(n, 4, device="cuda"), n, 1, 4, torch.ones(4, device="cuda"), dz, db=db)
+    assert abs(db.item() - (want.sum().item() - 2.0)) <= 1e-6
+    del z, y, dz
+    torch.cuda.empty_cache()
+
+
+@pytest.mark.gpu
+def test_head_gradient_of_the_widest_rows(ops):
+    """rows of 2^31 - 8 values: the last step past a row must not wrap either"""
+    d = (1 << 31) - 8
+    w = torch.zeros(d, device="cuda")
+    w[-8:] = torch.arange(1.0, 9.0, device="cuda")
+    w[:4] = 3.0
+    dh = torch.full((2, d), 7.0, dtype=F16, device="cuda")
+    ops.pool_score_backward(torch.empty(2, d, device="cuda"), 2, 1, d, w, torch.tensor([1.0, -2.0], device="cuda"), dh)
+    for row, z in enumerate((1.0, -2.0)):
+        assert (dh[row, :4] == 3.0 * z).all() and (dh[row, 4:-8] == 0).all() and (dh[row, -8:] == z * w[-8:]).all()
+    del w, dh
+    torch.cuda.empty_cache()

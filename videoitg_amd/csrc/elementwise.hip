@@ -697,7 +697,7 @@ __global__ __launch_bounds__(1024) void bce_loss_kernel(const float* __restrict_
     __shared__ float red[32];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     float pos = 0.f;
-    for (int i = tid; i < n; i += blockDim.x) pos += y[i];
+    for (long i = tid; i < n; i += blockDim.x) pos += y[i];         // (long: the last step past n must not wrap)
     pos = wave_sum(pos);
     if (lane == 0) red[wave] = pos;
     __syncthreads();
@@ -707,7 +707,7 @@ __global__ __launch_bounds__(1024) void bce_loss_kernel(const float* __restrict_
     const float neg = (float)n - pos;
     const float pw = fminf(5.0f, sqrtf(neg / fmaxf(1.0f, pos)));
     float acc = 0.f;
-    for (int i = tid; i < n; i += blockDim.x) {
+    for (long i = tid; i < n; i += blockDim.x) {
         const float xi = x[i], yi = y[i];
         const float sp = log1pf(expf(-fabsf(xi))) + fmaxf(-xi, 0.0f);       // softplus(-x), stable
         acc += (1.0f - yi) * xi + (1.0f + (pw - 1.0f) * yi) * sp;

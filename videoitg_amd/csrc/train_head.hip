@@ -104,18 +104,18 @@ __device__ __forceinline__ double block_sum_1024(double v, double* red) {
     return v;
 }
 
-// one block: n is the number of frames of a batch (hundreds), the call is launch latency
+// one block: n is the number of frames of a batch (hundreds), the call is launch latency.  (long indices here and below: the last step past n must not wrap)
 __global__ __launch_bounds__(1024) void bce_loss_backward_kernel(const float* __restrict__ z, const float* __restrict__ y, int n, float scale,
                                                                  float* __restrict__ out2, float* __restrict__ dz) {
     __shared__ double red[16];
     double pos = 0.0;
-    for (int i = threadIdx.x; i < n; i += 1024) pos += y[i];
+    for (long i = threadIdx.x; i < n; i += 1024) pos += y[i];
     pos = block_sum_1024(pos, red);
     const float fpos = (float)pos;
     const float pw = fminf(5.0f, sqrtf(((float)n - fpos) / fmaxf(1.0f, fpos)));
     const float g = scale / (float)n;
     double loss = 0.0;
-    for (int i = threadIdx.x; i < n; i += 1024) {
+    for (long i = threadIdx.x; i < n; i += 1024) {
         const float zi = z[i], yi = y[i];
         const float e = expf(-fabsf(zi)), r = 1.0f / (1.0f + e);
         const float p = zi >= 0.f ? r : e * r, q = zi >= 0.f ? e * r : r;        // sigmoid(z), sigmoid(-z): no cancellation on either side
@@ -143,7 +143,7 @@ __global__ __launch_bounds__(256) void pool_score_backward_kernel(const float* _
         float acc[4] = {0.f, 0.f, 0.f, 0.f};
         if (c < D && dw) {
 #pragma unroll 4
-            for (int t = grp; t < frames; t += 16) {
+            for (long t = grp; t < frames; t += 16) {
                 float v[4];
                 load_vec<float, 4>(pooled + t * ldp + c, v);
                 const float d = dz[t];
@@ -154,7 +154,7 @@ __global__ __launch_bounds__(256) void pool_score_backward_kernel(const float* _
         store_vec<float, 4>(&part[grp][q * 4], acc);
         double sum = 0.0;
         if (db && blockIdx.x == 0)
-            for (int t = threadIdx.x; t < frames; t += 256) sum += dz[t];
+            for (long t = threadIdx.x; t < frames; t += 256) sum += dz[t];
 #pragma unroll
         for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
         if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = sum;
@@ -175,7 +175,7 @@ __global__ __launch_bounds__(256) void pool_score_backward_kernel(const float* _
     const long t = id / slices;
     const int j0 = id % slices * DH_ROWS, j1 = min(j0 + DH_ROWS, tokens);
     const float d = dz[t] / (float)tokens;
-    for (int c = threadIdx.x * V; c < D; c += 256 * V) {
+    for (long c = threadIdx.x * V; c < D; c += 256 * V) {
         float v[V];
         load_vec<float, V>(w + c, v);
 #pragma unroll
