@@ -72,3 +72,34 @@ def test_head_gradient_of_the_widest_rows(ops):
         assert (dh[row, :4] == 3.0 * z).all() and (dh[row, 4:-8] == 0).all() and (dh[row, -8:] == z * w[-8:]).all()
     del w, dh
     torch.cuda.empty_cache()
+
+
+def test_dispatcher_form_of_clipping_refuses_what_the_binding_refuses():
+    from videoitg_amd._lib import VitgError
+    from videoitg_amd.torch_ops import K
+    g = [torch.ones(3)]
+    for call in (lambda: K.clip_grad_norm(g, None, outs=[torch.zeros(3)]), lambda: K.clip_grad_norm([], 1.0), lambda: K.clip_grad_norm(iter(()), None)):
+        with pytest.raises(VitgError):
+            call()
+
+
+@pytest.mark.gpu
+def test_dispatcher_form_of_clipping_takes_every_argument(ops):
+    from videoitg_amd.torch_ops import K
+    make = lambda: [torch.arange(1.0, 3000.0, device="cuda").to(F16), torch.arange(7.0, device="cuda")]      # noqa: E731
+    zeros = lambda: [torch.zeros_like(t) for t in make()]                                                     # noqa: E731
+    with pytest.raises(Exception, match="no outs"):
+        K.clip_grad_norm(make(), None, outs=zeros())
+    ws = torch.empty(4096, dtype=torch.uint8, device="cuda")
+    for max_norm in (0.5, None):
+        for outs in (False, True):
+            if outs and max_norm is None:
+                continue
+            for norm in (False, True):
+                for workspace in (None, ws):
+                    got, want, o, p = make(), make(), zeros(), zeros()
+                    slot = torch.full((1,), -1.0, device="cuda") if norm else None
+                    a = K.clip_grad_norm(iter(got), max_norm, outs=iter(o) if outs else None, scale=0.25, norm=slot, workspace=workspace)
+                    b = ops.clip_grad_norm(want, max_norm, outs=p if outs else None, scale=0.25)
+                    assert torch.equal(a, b) and (not norm or a is slot)
+                    assert all(torch.equal(x, y) for x, y in zip(got + o, want + p))

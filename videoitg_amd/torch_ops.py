@@ -18,7 +18,7 @@ aliasing behaviour.
 Names are the build's choice: patchify, gemm, layernorm, rmsnorm, rope_, attention, bilinear_pool,
 gather_rows, embed_gather, pool_score, rank, preprocess_u8, bce_loss, quant_rows_fp8, norm_quant_fp8, gemm_fp8, gemm_fp8_mx,
 gemm_res16 / layernorm16 / bilinear_pool16 (the tower's 16-bit residual stream),
-embed_lookup / embed_backward, swiglu / swiglu_backward, pool_score_save / bce_loss_backward / pool_score_backward, grad_norm / clip_grad_norm(_) (training).
+embed_lookup / embed_backward, swiglu / swiglu_backward, pool_score_save / bce_loss_backward / pool_score_backward, grad_norm / clip_grad_norm(_, _into) (training).
 """
 from __future__ import annotations
 
@@ -215,6 +215,11 @@ _def("clip_grad_norm(Tensor[] grads, Tensor(a!)[] outs, float max_norm, float sc
 _def("clip_grad_norm_(Tensor(a!)[] grads, float max_norm, float scale=1.0) -> Tensor",
      lambda grads, max_norm, scale=1.0: _raw.clip_grad_norm(grads, max_norm, scale=scale),
      lambda grads, max_norm, scale=1.0: grads[0].new_empty(1, dtype=torch.float32))
+
+_def("clip_grad_norm_into(Tensor[] grads, Tensor(a!)[] outs, Tensor(b!) norm, float? max_norm, float scale=1.0, Tensor(c!)? workspace=None) -> ()",
+     lambda grads, outs, norm, max_norm, scale=1.0, workspace=None:
+         (_raw.clip_grad_norm(grads, max_norm, outs=None if max_norm is None else outs, scale=scale, norm=norm, workspace=workspace), None)[1],
+     lambda *a, **k: None)
 
 # ---- call-compatible namespace for the engine (same signatures as videoitg_amd.ops) ------------------------------------
 _ops = torch.ops.videoitg
@@ -441,10 +446,18 @@ class _Namespace:
         _ops.pool_score_backward(pooled, frames, tokens_per_frame, d, w, dlogits, dh, dw, db, accumulate)
 
     @staticmethod
-    def clip_grad_norm(grads, max_norm, *, outs=None, scale=1.0):
+    def clip_grad_norm(grads, max_norm, *, outs=None, scale=1.0, norm=None, workspace=None):
+        grads = list(grads)
+        if not grads or (max_norm is None and outs is not None):
+            return _raw.clip_grad_norm(grads, max_norm, outs=outs)           # (refused there)
+        if norm is not None or workspace is not None:
+            if norm is None:
+                norm = grads[0].new_empty(1, dtype=torch.float32)
+            _ops.clip_grad_norm_into(grads, [] if max_norm is None else grads if outs is None else list(outs), norm, max_norm, scale, workspace)
+            return norm
         if max_norm is None:
             return _ops.grad_norm(grads, scale)
-        return _ops.clip_grad_norm_(grads, max_norm, scale) if outs is None else _ops.clip_grad_norm(grads, outs, max_norm, scale)
+        return _ops.clip_grad_norm_(grads, max_norm, scale) if outs is None else _ops.clip_grad_norm(grads, list(outs), max_norm, scale)
 
 
 K = _Namespace()
@@ -453,4 +466,4 @@ OP_NAMES: List[str] = ["patchify", "gemm", "gemm_splitk", "gemm_splitk16", "laye
                        "gemm_res16", "layernorm16", "bilinear_pool16", "patch_embed16", "norm_quant_fp8_16", "gemm_fp8_res16",
                        "norm_split", "rope_split_", "bilinear_pool_split", "gemm_split16", "attention_split",
                        "embed_lookup", "embed_backward", "swiglu", "swiglu_backward", "pool_score_save", "bce_loss_backward", "pool_score_backward",
-                       "grad_norm", "clip_grad_norm", "clip_grad_norm_"] + (["gemm_streamk"] if _raw._lib.PROFILING else [])
+                       "grad_norm", "clip_grad_norm", "clip_grad_norm_", "clip_grad_norm_into"] + (["gemm_streamk"] if _raw._lib.PROFILING else [])
