@@ -103,3 +103,51 @@ def test_dispatcher_form_of_clipping_takes_every_argument(ops):
                     b = ops.clip_grad_norm(want, max_norm, outs=p if outs else None, scale=0.25)
                     assert torch.equal(a, b) and (not norm or a is slot)
                     assert all(torch.equal(x, y) for x, y in zip(got + o, want + p))
+
+
+def shifted(t, ld=0):
+    """the same values 16 bytes behind a 32-byte boundary, rows `ld` apart"""
+    rows, cols = t.shape if t.dim() == 2 else (1, t.numel())
+    ld = max(ld, cols)
+    flat = torch.zeros(rows * ld + 64, dtype=t.dtype, device="cuda")
+    assert flat.data_ptr() % 32 == 0
+    out = torch.as_strided(flat, (rows, cols), (ld, 1), 16 // t.element_size())
+    out.copy_(t.view(rows, cols))
+    return out if t.dim() == 2 else out[0]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("half", [BF16, F16])
+def test_fp32_operands_16_bytes_behind_a_32_byte_boundary(ops, half):
+    """eight values of a lane are two 16-byte accesses: 16-byte aligned rows of fp32 give the bits of fully aligned ones"""
+    g = torch.Generator(device="cuda").manual_seed(3)
+    rand = lambda *s, dtype=F32: torch.randn(*s, generator=g, device="cuda").to(dtype)      # noqa: E731
+    ids = torch.randint(-1, 40, (300,), generator=g, device="cuda")
+    table, dout = rand(40, 264), rand(300, 264)
+    for dtype in (half, F32):
+        same = ops.embed_lookup(ids, shifted(table), shifted(torch.zeros(300, 264, dtype=dtype)))
+        assert torch.equal(same, ops.embed_lookup(ids, table, torch.zeros(300, 264, dtype=dtype, device="cuda")))
+        for add in (False, True):
+            a, b = shifted(table.to(dtype)), table.to(dtype)
+            ops.embed_backward(ids, shifted(dout), a, accumulate=add)
+            ops.embed_backward(ids, dout, b, accumulate=add)
+            assert torch.equal(a, b)
+    x, gu, up = rand(20, 128, dtype=half), rand(20, 256, dtype=half), rand(20, 128, dtype=half)
+    a, b = shifted(torch.ones(256, 128)), torch.ones(256, 128, device="cuda")
+    w = rand(256, 128, dtype=half)
+    ops.swiglu_backward(up, gu, x, w, dw=a, accumulate=True)
+    ops.swiglu_backward(up, gu, x, w, dw=b, accumulate=True)
+    assert torch.equal(a, b)
+    for frames, tokens in ((9, 5), (3, 150)):            # one block a frame; rows over several blocks
+        h, hw, bias = rand(frames * tokens, 520, dtype=half), rand(520), rand(1)
+        z, zs, p, ps = (torch.empty(frames, device="cuda"), torch.empty(frames, device="cuda"), torch.empty(frames, 520, device="cuda"), shifted(torch.zeros(frames, 520), 524))
+        ops.pool_score_save(h, frames, tokens, 520, hw, bias, z, p)
+        ops.pool_score_save(h, frames, tokens, 520, shifted(hw), bias, zs, ps)
+        assert torch.equal(z, zs) and torch.equal(p, ps)
+        d, ds, dw, dws = torch.empty_like(h), torch.empty_like(h), torch.empty_like(hw), shifted(torch.zeros(520))
+        ops.pool_score_backward(p, frames, tokens, 520, hw, z, d, dw=dw)
+        ops.pool_score_backward(ps, frames, tokens, 520, shifted(hw), z, ds, dw=dws)
+        assert torch.equal(d, ds) and torch.equal(dw, dws)
+    t = shifted(rand(70000))
+    u = t.clone()
+    assert torch.equal(ops.clip_grad_norm([t], 1.0), ops.clip_grad_norm([u], 1.0)) and torch.equal(t, u)

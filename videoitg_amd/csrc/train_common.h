@@ -6,8 +6,13 @@
 
 namespace vitg {
 
-// V consecutive elements of type T <-> fp32 values; p aligned to the vector
-template <typename T, int V> struct Pack { typedef T type __attribute__((ext_vector_type(V))); };
+// V consecutive elements of type T <-> fp32 values; p aligned to the vector, or to 16 bytes where the vector is longer (eight fp32 values: two 16-byte accesses) -
+// what the entry points check
+template <typename T, int V> struct Pack {
+    typedef T type __attribute__((ext_vector_type(V), aligned(sizeof(T) * V < 16 ? sizeof(T) * V : 16)));
+};
+static_assert(alignof(Pack<float, 8>::type) == 16 && alignof(Pack<bf16_t, 8>::type) == 16 && alignof(Pack<f16_t, 4>::type) == 8 && sizeof(Pack<float, 8>::type) == 32,
+              "no access asks for more than the checked alignment");
 template <typename T, int V> __device__ __forceinline__ void load_vec(const T* p, float (&v)[V]) {
     const typename Pack<T, V>::type x = *(const typename Pack<T, V>::type*)p;
 #pragma unroll
