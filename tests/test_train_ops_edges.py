@@ -151,3 +151,66 @@ def test_fp32_operands_16_bytes_behind_a_32_byte_boundary(ops, half):
     t = shifted(rand(70000))
     u = t.clone()
     assert torch.equal(ops.clip_grad_norm([t], 1.0), ops.clip_grad_norm([u], 1.0)) and torch.equal(t, u)
+
+
+def test_shared_memory_is_found_byte_for_byte():
+    """every pair of row blocks in a small buffer against the sets of bytes they hold; only rows of two pitches may be refused without need"""
+    from videoitg_amd import ops
+    checked = refused = 0
+    flat = torch.zeros(96, dtype=F16)
+    views = [torch.as_strided(flat, (rows, cols), (ld, 1), at) for rows in (1, 2, 3) for ld in (8, 12) for cols in (2, 5, 8, 12) if cols <= ld for at in (0, 1, 3, 7, 8, 13, 24, 30)
+             if at + (rows - 1) * ld + cols <= 96]
+    held = [{v.storage_offset() + i * v.stride(0) + j for i in range(v.shape[0]) for j in range(v.shape[1])} for v in views]
+    item = lambda v: ("v", v.data_ptr(), v.data_ptr() + 2 * ((v.shape[0] - 1) * v.stride(0) + v.shape[1]), v)      # noqa: E731
+    items = [item(v) for v in views]
+    for v, p, a in zip(views, items, held):
+        for u, q, b in zip(views, items, held):
+            meet = ops._meet(p, q)
+            if a & b:
+                assert meet
+            elif meet:
+                assert v.shape[0] > 1 and u.shape[0] > 1 and v.stride(0) != u.stride(0)
+                refused += 1
+            checked += 1
+    assert checked > 5000 and refused < checked / 10
+    assert not ops._meet(("empty", 100, 100), ("v", 50, 150)) and ops._meet(("a", 100, 120), ("b", 119, 130)) and not ops._meet(("a", 100, 120), ("b", 120, 130))
+
+
+@pytest.mark.gpu
+def test_column_slices_of_one_buffer(ops):
+    """operands and results side by side in one buffer give the bits of separate ones; slices that share a column are refused"""
+    from videoitg_amd._lib import VitgError
+    g = torch.Generator(device="cuda").manual_seed(8)
+    rand = lambda *s, dtype=F32: torch.randn(*s, generator=g, device="cuda").to(dtype)      # noqa: E731
+    for m, k, n in ((9, 128, 192), (70, 64, 320), (300, 256, 832), (600, 1024, 128)):
+        x, w, dout = rand(m, k, dtype=BF16), rand(n, k, dtype=BF16), rand(m, n // 2, dtype=BF16)
+        act, gu, dx, dw = x.new_empty(m, n // 2), x.new_empty(m, n), torch.empty_like(x), torch.empty_like(w)
+        ops.swiglu(x, w, act, gu=gu)
+        ops.swiglu_backward(dout, gu, x, w, dx=dx, dw=dw)
+        rows = torch.full((m, 2 * k + 2 * n), 7.0, dtype=BF16, device="cuda")
+        xs, acts, gus, dxs, douts = rows.split([k, n // 2, n, k, n // 2], 1)
+        both = torch.full((n, 2 * k), 7.0, dtype=BF16, device="cuda")
+        ws, dws = both.split(k, 1)
+        xs.copy_(x), douts.copy_(dout), ws.copy_(w)
+        ops.swiglu(xs, ws, acts, gu=gus)
+        ops.swiglu_backward(douts, gus, xs, ws, dx=dxs, dw=dws)
+        for got, want in ((acts, act), (gus, gu), (dxs, dx), (dws, dw), (xs, x), (ws, w), (douts, dout)):
+            assert torch.equal(got, want)
+        with pytest.raises(VitgError, match="share memory"):
+            ops.swiglu(xs, ws, rows[:, k - 8:k - 8 + n // 2])
+    ids = torch.randint(-1, 50, (400,), generator=g, device="cuda")
+    one = rand(50, 2 * 96)
+    table, dtable = one.split(96, 1)
+    rows = rand(50, 2 * 96)[torch.arange(400, device="cuda") % 50]
+    out, dout = rows.split(96, 1)
+    want = ops.embed_lookup(ids, table.contiguous(), torch.empty(400, 96, device="cuda"))
+    grad = ops.embed_backward(ids, dout.contiguous(), torch.empty(50, 96, device="cuda"))
+    assert torch.equal(ops.embed_lookup(ids, table, out), want) and torch.equal(ops.embed_backward(ids, dout, dtable), grad)
+    h = rand(60 * 5, 2 * 264)
+    w, b, z, z2, pooled = rand(264), rand(1), torch.empty(60, device="cuda"), torch.empty(60, device="cuda"), torch.empty(60, 264, device="cuda")
+    ops.pool_score_save(h[:, :264].contiguous(), 60, 5, 264, w, b, z, pooled)
+    ops.pool_score_save(h[:, :264], 60, 5, 264, w, b, z2, pooled)
+    dh = torch.empty(300, 264, device="cuda")
+    ops.pool_score_backward(pooled, 60, 5, 264, w, z, dh)
+    ops.pool_score_backward(pooled, 60, 5, 264, w, z2, h[:, 264:])
+    assert torch.equal(z, z2) and torch.equal(h[:, 264:], dh)

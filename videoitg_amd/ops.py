@@ -699,15 +699,36 @@ def _workspace(workspace: Optional[torch.Tensor], need: int, idx: int):
     return workspace, workspace.data_ptr(), have
 
 
+def _meet(p, q) -> bool:
+    """whether two items (name, address, end, matrix or nothing) share memory.  Rows one pitch apart that keep to different columns of it - column slices of one
+    buffer - do not; rows of two pitches between each other's are taken as sharing"""
+    if p[1] > q[1]:
+        p, q = q, p
+    if p[1] == p[2] or q[1] == q[2] or q[1] >= p[2]:
+        return False
+    pitch, widths = 0, []
+    for _, begin, end, *t in (p, q):
+        if t and t[0].shape[0] > 1:
+            size = _SIZE[t[0].dtype]
+            if pitch and pitch != t[0].stride(0) * size:
+                return True
+            pitch = t[0].stride(0) * size
+            widths.append(t[0].shape[1] * size)
+        else:
+            widths.append(end - begin)
+    if not pitch:
+        return True
+    column = (q[1] - p[1]) % pitch                       # where q's rows begin, from the begin of p's
+    return column < widths[0] or column + widths[1] > pitch
+
+
 def _distinct(outputs, inputs=()):
-    """no output of a call shares memory with an input or another output; items are (name, address, end)"""
-    for i, (n, a, z) in enumerate(outputs):
-        for m, b, y in outputs[i + 1:]:
-            if a < y and b < z:
-                _fail(f"{n} and {m} share memory")
-        for m, b, y in inputs:
-            if a < y and b < z:
-                _fail(f"{n} and {m} share memory")
+    """no output of a call shares memory with an input or another output; items are (name, address, end) or (name, address, end, matrix)"""
+    for i, out in enumerate(outputs):
+        a, z = out[1], out[2]
+        for other in (*outputs[i + 1:], *inputs):
+            if a < other[2] and other[1] < z and _meet(out, other):
+                _fail(f"{out[0]} and {other[0]} share memory")
 
 
 def embed_lookup(ids: torch.Tensor, table: torch.Tensor, out: torch.Tensor, *, scale: float = 1.0) -> torch.Tensor:
@@ -718,7 +739,7 @@ def embed_lookup(ids: torch.Tensor, table: torch.Tensor, out: torch.Tensor, *, s
     pi, ei = _vector(ids, "ids", n, torch.int64)
     pt, ldt, et = _matrix(table, "table", vocab, d, _FLOATS)
     po, ldo, eo = _matrix(out, "out", n, d, _FLOATS)
-    _distinct([("out", po, eo)], [("table", pt, et), ("ids", pi, ei)])
+    _distinct([("out", po, eo, out)], [("table", pt, et, table), ("ids", pi, ei)])
     _call_on(idx, "vitg_embed_lookup", pi, n, pt, _DT[table.dtype], ldt, vocab, d, scale, po, _DT[out.dtype], ldo)
     return out
 
@@ -747,7 +768,7 @@ def embed_backward(ids: torch.Tensor, dout: torch.Tensor, dtable: torch.Tensor, 
     pd, ldd, ed = _matrix(dout, "dout", n, d, _FLOATS)
     pt, ldt, et = _matrix(dtable, "dtable", vocab, d, _FLOATS)
     ws, pw, nw = _workspace(workspace, _plan_on(idx, embed_backward_plan, n, d), idx)
-    _distinct([("dtable", pt, et), ("workspace", pw, pw + nw)], [("dout", pd, ed), ("ids", pi, ei)])
+    _distinct([("dtable", pt, et, dtable), ("workspace", pw, pw + nw)], [("dout", pd, ed, dout), ("ids", pi, ei)])
     _call_on(idx, "vitg_embed_backward", pi, n, pd, _DT[dout.dtype], ldd, vocab, d, scale, pt, _DT[dtable.dtype], ldt, 1 if accumulate else 0, pw, nw)
     return dtable
 
@@ -761,11 +782,11 @@ def swiglu(x: torch.Tensor, w: torch.Tensor, out: torch.Tensor, *, gu: Optional[
     px, ldx, ex = _matrix(x, "x", m, k, _HALVES)
     pw, ldw, ew = _matrix(w, "w", nn, k, (dt,))
     po, ldo, eo = _matrix(out, "out", m, nn // 2, (dt,))
-    outs, pg, ldg = [("out", po, eo)], 0, 0
+    outs, pg, ldg = [("out", po, eo, out)], 0, 0
     if gu is not None:
         pg, ldg, eg = _matrix(gu, "gu", m, nn, (dt,))
-        outs.append(("gu", pg, eg))
-    _distinct(outs, (("x", px, ex), ("w", pw, ew)))
+        outs.append(("gu", pg, eg, gu))
+    _distinct(outs, (("x", px, ex, x), ("w", pw, ew, w)))
     _call_on(idx, "vitg_swiglu", px, ldx, pw, ldw, m, nn, k, _DT[dt], po, ldo, pg, ldg)
     return out
 
@@ -791,16 +812,16 @@ def swiglu_backward(dout: torch.Tensor, gu: torch.Tensor, x: torch.Tensor, w: to
     outs, pdx, lddx, pdw, lddw, dwt = [], 0, 0, 0, 0, dt
     if dx is not None:
         pdx, lddx, e = _matrix(dx, "dx", m, k, (dt,))
-        outs.append(("dx", pdx, e))
+        outs.append(("dx", pdx, e, dx))
     if dw is not None:
         dwt = dw.dtype
         pdw, lddw, e = _matrix(dw, "dw", nn, k, (dt, torch.float32))
-        outs.append(("dw", pdw, e))
+        outs.append(("dw", pdw, e, dw))
     if not outs:
         return
     ws, pws, nws = _workspace(workspace, _plan_on(idx, swiglu_backward_plan, m, nn, k, dx is not None, dw is not None), idx)
     outs.append(("workspace", pws, pws + nws))
-    _distinct(outs, (("dout", pd, ed), ("gu", pg, eg), ("x", px, ex), ("w", pw, ew)))
+    _distinct(outs, (("dout", pd, ed, dout), ("gu", pg, eg, gu), ("x", px, ex, x), ("w", pw, ew, w)))
     _call_on(idx, "vitg_swiglu_backward", pd, ldd, pg, ldg, px, ldx, pw, ldw, m, nn, k, _DT[dt], pdx, lddx, pdw, lddw, _DT[dwt], 1 if accumulate else 0, pws, nws)
 
 
@@ -813,7 +834,7 @@ def pool_score_save(h: torch.Tensor, frames: int, tokens_per_frame: int, d: int,
     ph, ldh, eh = _matrix(h, "h", frames * tokens_per_frame, d, _FLOATS)
     pp, ldp, ep = _matrix(pooled, "pooled", frames, d, (torch.float32,))
     (pw, ew), (pb, eb), (pl, el) = _vector(w, "w", d, torch.float32), _vector(b, "b", 1, torch.float32), _vector(logits, "logits", frames, torch.float32)
-    _distinct([("logits", pl, el), ("pooled", pp, ep)], (("h", ph, eh), ("w", pw, ew), ("b", pb, eb)))
+    _distinct([("logits", pl, el), ("pooled", pp, ep, pooled)], (("h", ph, eh, h), ("w", pw, ew), ("b", pb, eb)))
     _call_on(idx, "vitg_pool_score_save", ph, _DT[h.dtype], ldh, frames, tokens_per_frame, d, pw, pb, pl, pp, ldp)
     return logits
 
@@ -850,14 +871,14 @@ def pool_score_backward(pooled: torch.Tensor, frames: int, tokens_per_frame: int
     if dh is not None:
         hdt = dh.dtype
         ph, ldh, e = _matrix(dh, "dh", frames * tokens_per_frame, d, _FLOATS)
-        outs.append(("dh", ph, e))
+        outs.append(("dh", ph, e, dh))
     if dw is not None:
         pdw, e = _vector(dw, "dw", d, torch.float32)
         outs.append(("dw", pdw, e))
     if db is not None:
         pdb, e = _vector(db, "db", 1, torch.float32)
         outs.append(("db", pdb, e))
-    _distinct(outs, (("pooled", pp, ep), ("w", pw, ew), ("dlogits", pz, ez)))
+    _distinct(outs, (("pooled", pp, ep, pooled), ("w", pw, ew), ("dlogits", pz, ez)))
     _call_on(idx, "vitg_pool_score_backward", pp, ldp, frames, tokens_per_frame, d, pw, pz, ph, _DT[hdt], ldh, pdw, pdb, 1 if accumulate else 0)
 
 
