@@ -214,3 +214,19 @@ def test_column_slices_of_one_buffer(ops):
     ops.pool_score_backward(pooled, 60, 5, 264, w, z, dh)
     ops.pool_score_backward(pooled, 60, 5, 264, w, z2, h[:, 264:])
     assert torch.equal(z, z2) and torch.equal(h[:, 264:], dh)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("low,high", [(3.0, 6.0), (9.0, 11.0), (14.0, 30.0), (60.0, 90.0)])
+def test_loss_of_scores_that_are_right(ops, low, high):
+    """every frame on its own side: the loss is a sum of exponentials.  A term is off by the rounding of the logarithm (2 units), the exponential (2 units; its argument is exact),
+    a product and two sums, half a unit of 2^-23 each, the weight by 3 units: 2^-20 together"""
+    g = torch.Generator().manual_seed(int(low))
+    y = (torch.rand(700, generator=g) < 0.3).float()
+    z = (torch.rand(700, generator=g) * (high - low) + low) * (2 * y - 1)
+    z64, y64 = z.double(), y.double()
+    pos = float(y64.sum())
+    pw = min(5.0, ((700 - pos) / max(1.0, pos)) ** 0.5)
+    want = -(pw * y64 * torch.nn.functional.logsigmoid(z64) + (1 - y64) * torch.nn.functional.logsigmoid(-z64)).mean().item()
+    loss, weight, dz = ops.bce_loss_backward(z.cuda(), y.cuda())
+    assert abs(loss.item() / want - 1) <= 2.0 ** -20

@@ -119,8 +119,8 @@ __global__ __launch_bounds__(1024) void bce_loss_backward_kernel(const float* __
         const float zi = z[i], yi = y[i];
         const float e = expf(-fabsf(zi)), r = 1.0f / (1.0f + e);
         const float p = zi >= 0.f ? r : e * r, q = zi >= 0.f ? e * r : r;        // sigmoid(z), sigmoid(-z): no cancellation on either side
-        const float sp = log1pf(e) + fmaxf(-zi, 0.0f);                           // softplus(-z)
-        loss += (1.0f - yi) * zi + (1.0f + (pw - 1.0f) * yi) * sp;
+        const float t = log1pf(e);                       // softplus(z) = t + max(z, 0), softplus(-z) = t + max(-z, 0): a sum of terms of one sign -
+        loss += (1.0f - yi) * (t + fmaxf(zi, 0.0f)) + pw * yi * (t + fmaxf(-zi, 0.0f));      // (1 - y) z + softplus(-z) cancels where the scores are right
         dz[i] = g * ((1.0f - yi) * p - pw * yi * q);
     }
     loss = block_sum_1024(loss, red);
