@@ -332,8 +332,8 @@ int vitg_pool_score_backward(const float* pooled, long ldp, int frames, int toke
 
 /* Global gradient norm over `count` tensors (HOST arrays of device pointers, element counts and dtype codes; contiguous tensors of fp32, fp16, bf16, mixed):
  * norm[0] = |scale| * sqrt(sum g^2) and, unless outs is NULL, outs[i] = grads[i] * scale * min(1, max_norm / (norm + 1e-6)); outs[i] may be grads[i], and
- * otherwise overlaps no tensor of the call.  Squares are summed in fp64.  An infinite norm gives factor 0, a NaN norm NaN, as the formula says; max_norm =
- * infinity scales only.  The addresses travel as kernel arguments: a captured call replays on the same tensors.  workspace: vitg_clip_grad_plan bytes,
+ * otherwise overlaps no tensor of the call.  Squares are summed in fp64.  An infinite norm gives factor 0, a NaN norm NaN, as the formula says (a finite
+ * one beyond fp32 reads infinity in norm[0], while the factor comes from its fp64 value); max_norm = infinity scales only.  The addresses travel as kernel arguments: a captured call replays on the same tensors.  workspace: vitg_clip_grad_plan bytes,
  * 8-byte aligned.  (The reference's Trainer clips with max_grad_norm over all parameters of the model.) */
 int vitg_clip_grad_plan(int count, const long* numel, const int* dtype, long* workspace_bytes);
 int vitg_clip_grad(int count, const void* const* grads, void* const* outs, const long* numel, const int* dtype, float scale, float max_norm, float* norm,

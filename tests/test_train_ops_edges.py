@@ -230,3 +230,21 @@ def test_loss_of_scores_that_are_right(ops, low, high):
     want = -(pw * y64 * torch.nn.functional.logsigmoid(z64) + (1 - y64) * torch.nn.functional.logsigmoid(-z64)).mean().item()
     loss, weight, dz = ops.bce_loss_backward(z.cuda(), y.cuda())
     assert abs(loss.item() / want - 1) <= 2.0 ** -20
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("max_norm", [1.0, 1e-3, 1e-12, 1e-30])
+def test_clipping_by_a_factor_below_the_normal_numbers(ops, max_norm):
+    """norms of 1e39 and more: the factor has no fp32 value of 24 bits, the results do"""
+    g = torch.Generator().manual_seed(4)
+    grads = [(torch.rand(3000, generator=g) + 0.1) * 3e38, ((torch.rand(517, generator=g) + 0.1) * 3e38).to(BF16), torch.randn(5, generator=g) * 1e30, torch.full((3,), -1e20)]
+    limit = float(torch.tensor(max_norm, dtype=F32))
+    norm = sum(float(t.double().square().sum()) for t in grads) ** 0.5
+    assert limit / norm < 1.2e-38
+    dev = [t.cuda() for t in grads]
+    assert ops.clip_grad_norm(dev, max_norm).item() == float("inf")       # (beyond fp32)
+    for t, o in zip(grads, dev):
+        want = t.double() * (limit / (norm + 1e-6))
+        half, least = (2.0 ** -8, 2.0 ** -133) if t.dtype == BF16 else (2.0 ** -24, 2.0 ** -149)
+        bound = want.abs() * (4 * 2.0 ** -24 + half * 1.001) + least
+        assert ((o.double().cpu() - want).abs() <= bound).all()

@@ -93,8 +93,18 @@ __global__ __launch_bounds__(CLIP_THREADS) void grad_sumsq_kernel(const ClipArgs
     if (threadIdx.x == 0) sums[blockIdx.x] = s;
 }
 
+// a factor below fp32's normal numbers (norms beyond 1e38, tiny limits) keeps its 24 bits as factor = first * second with a power of two for second: first * v does
+// not overflow, and where it is subnormal the result is zero.  Ordinary factors have second = 1
+struct ClipFactor { float first, second; };
+__device__ __forceinline__ ClipFactor clip_factor(double f) {
+    const double a = fabs(f);
+    if (a < 0x1p-186) return {(float)(f * 0x1p126), 0x1p-126f};
+    if (a < 0x1p-100) return {(float)(f * 0x1p64), 0x1p-64f};
+    return {(float)f, 1.0f};
+}
+
 template <bool AROUND, typename T>
-__device__ __forceinline__ void clip_scale_piece(const T* p, T* q, long count, float factor, int tid) {
+__device__ __forceinline__ void clip_scale_piece(const T* p, T* q, long count, const ClipFactor f, int tid) {
     constexpr int V = 16 / sizeof(T);
     long done = 0;
     if ((((uintptr_t)p | (uintptr_t)q) & 15) == 0) {
@@ -107,7 +117,7 @@ __device__ __forceinline__ void clip_scale_piece(const T* p, T* q, long count, f
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
 #pragma unroll
-                for (int e = 0; e < V; ++e) v[u][e] *= factor;
+                for (int e = 0; e < V; ++e) v[u][e] = v[u][e] * f.first * f.second;
                 store_stream<T, V, AROUND>(q + i + u * CLIP_THREADS * V, v[u]);
             }
         }
@@ -115,11 +125,11 @@ __device__ __forceinline__ void clip_scale_piece(const T* p, T* q, long count, f
             float v[V];
             load_vec<T, V>(p + i, v);
 #pragma unroll
-            for (int e = 0; e < V; ++e) v[e] *= factor;
+            for (int e = 0; e < V; ++e) v[e] = v[e] * f.first * f.second;
             store_vec<T, V>(q + i, v);
         }
     }
-    for (long i = done + tid; i < count; i += CLIP_THREADS) q[i] = (T)((float)p[i] * factor);
+    for (long i = done + tid; i < count; i += CLIP_THREADS) q[i] = (T)((float)p[i] * f.first * f.second);
 }
 
 // the norm of all tensors from the sums of pass 1 (every block adds them in the same order)
@@ -137,12 +147,12 @@ __global__ __launch_bounds__(CLIP_THREADS) void grad_scale_kernel(const ClipArgs
     if (norm_out && blockIdx.x == 0 && threadIdx.x == 0) *norm_out = (float)norm;
     // max_norm / inf = 0 and NaN stays NaN, as dividing by the norm says: an overflowed step shows in the norm AND in the gradients.  max_norm = inf: no limit
     const double clip = max_norm == INFINITY ? 1.0 : (double)max_norm / (norm + 1e-6);
-    const float factor = (float)((double)scale * (clip < 1.0 ? clip : clip != clip ? clip : 1.0));
+    const ClipFactor factor = clip_factor((double)scale * (clip < 1.0 ? clip : clip != clip ? clip : 1.0));
     const int pieces = a.count ? a.piece0[a.count] : 0;
     // from the end: what pass 1 read last is still in the last-level cache
     for (int p = pieces - 1 - (int)blockIdx.x; p >= 0; p -= gridDim.x) {
         const int t = clip_find(a, p);
-        if (factor == 1.0f && a.in[t] == a.out[t]) continue;                    // in place and nothing to scale
+        if (factor.first == 1.0f && a.in[t] == a.out[t]) continue;              // in place and nothing to scale (second is 1 then)
         const int esize = a.dtype[t] == DT_F32 ? 4 : 2;
         const long per = CLIP_PIECE / esize, at = (long)(p - a.piece0[t]) * per, count = min(per, a.numel[t] - at);
         if (a.dtype[t] == DT_BF16) clip_scale_piece<AROUND>((const bf16_t*)a.in[t] + at, (bf16_t*)a.out[t] + at, count, factor, threadIdx.x);
