@@ -27,7 +27,7 @@ if [ "${1:-}" = "--exp" ]; then
   OBJ="$HERE/build_exp_${NAME}"
   DEFS="-DVITG_EXP=1"
 fi
-# VITG_CLEAN=1: compile every source from scratch (the default reuses objects newer than their sources and shared headers)
+# VITG_CLEAN=1: compile every source from scratch (the default reuses objects newer than their sources, the shared headers and this script)
 if [ "${VITG_CLEAN:-0}" != "0" ]; then rm -rf "$OBJ" "$OUT"; fi
 mkdir -p "$OBJ"
 pids=()

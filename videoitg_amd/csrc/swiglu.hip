@@ -9,9 +9,9 @@
 // out of its elementwise kernel in both orders and X passes through a tile transpose in front of the ordinary NT GEMM.  dGU is rounded to the 16-bit type once -
 // the matrix pipe's operand type - and every sum over it is fp32.
 //
-// Measured at 3584 x 37888 (bf16; large library products of these shapes run at 1 307 - 1 436 TFLOP/s): one row 49 us = 5.6 TB/s of W; 12 860 rows with
+// Measured at 3584 x 37888 (bf16; large library products of these shapes run at 1 307 - 1 436 TFLOP/s): one row 49 us = 5.6 TB/s of W (the kernel; 59 the call, back to back); 12 860 rows with
 // pre-activations 2.67 ms = 1 309 TFLOP/s; their backward 5.73 ms: 0.80 in front (4.1 GB, 5.2 TB/s), dX and dW 2.46 each = 1 420 TFLOP/s; 1 607 rows (fp16)
-// 0.88 ms: 0.08 + dX 0.43 (two shares, K-major) + dW 0.38 + the join 0.01.
+// 0.88 ms: 0.08 + dX 0.43 (320-row tiles, K-major, three shares: 1 920 rows are multiplied) + dW 0.38 + the join 0.01.
 #include "train_common.h"
 #include "gemm_common.h"
 
@@ -324,8 +324,9 @@ __global__ __launch_bounds__(256) void swiglu_rows_backward_kernel(const T* __re
     else dw_rows_block<T, TW, AROUND>((id - dx_blocks) % columns, (id - dx_blocks) / columns, dgut, Mp, X, ldx, M, N, K, dW, lddw, accumulate);
 }
 
-// rows that the three kernels take, against the GEMM forms at 3584 x 37888 (us): forward 61 - 74 at 1 - 16 rows, the 128-row tile 69 - 75 at 17 - 128;
-// dX 70 - 83 at 1 - 32, 110 at 64, the K-major GEMM 91 at 65; dW 50 at 1 - 32, the GEMM 59 - 67 with a transpose of X in front
+// rows that the three kernels take, against the GEMM forms beside them: whole calls back to back at 3584 x 37888, bf16, over weights that do not fit the last-level
+// cache (us): forward 59 / 65 / 73 at 1 / 8 / 16 rows, the 128x128 tile 67 / 71 / 80 at 17 / 64 / 128; dX and dW of one call 154 at 1 - 32 rows, the GEMM forms 158 / 161
+// at 33 / 64; with the fp32 dW added 314 - 324 against 362 - 364.  (dX alone: 69 - 82 at 1 - 32 against 60 at 33; dW alone 78 - 87 against 70.)
 constexpr int FWD_ROWS = 16, BWD_ROWS = 32;
 
 // shares of W's rows per 128 columns of dX: three blocks per CU, at least 4 steps of 32 rows per wave
@@ -337,8 +338,10 @@ static int dx_shares(int N, int K) {
 // dX = dGU W for more rows: the GEMM with the K-major weight operand (gemm_mi16.hip), or a tile transpose of W in front of the NT GEMM, whose main loop is faster
 // (12 860 rows: 2.43 + 0.12 ms against 2.78; 1 607 rows: 0.41 + 0.12 against 0.43).  Either may split its contraction (N) into fp32 partials where one round
 // of tiles leaves CUs idle.  Estimated in microseconds: a 64-deep K-tile of a 256x256 tile takes 1.7 K-major and 1.48 NT (all CUs busy; the wide NT tiles are
-// 10 % and 5 % better per flop), the transpose moves its bytes at 4.6 TB/s.  Small problems run on the ring kernel (gemm_ring.hip).  Against every alternative
-// forced in turn on 40 shapes (448 .. 3584 x 1024 .. 37888, 40 .. 4 096 rows) the estimate's choice was within 10 % of the best.
+// 10 % and 5 % better per flop), the transpose moves its bytes at 4.6 TB/s.  Small problems run on the ring kernel (gemm_ring.hip).  Most alternatives were
+// forced in turn on 41 shapes (448 .. 3584 x 1024 .. 37888, 40 .. 4 096 rows; dX and dW): in 68 of 82 products the choice is among the five fastest and within
+// 8 % of the best.  The others take a share count that the sweep left out, or lie behind it: 448 x 4544, 4 096 rows 15 % or more (K-major, eight shares, where the ring
+// kernel in two takes 46 us - join_us prices 117 MB of partials as if they stayed in the cache).
 enum { DX_KMAJOR, DX_TRANSPOSED, DX_RING };
 struct DxPlan { int kind, bm, splits; };
 // a 64-deep K-tile of the 128x128 ring kernel: 0.35 us alone, 0.7 with a block on every CU (L2)

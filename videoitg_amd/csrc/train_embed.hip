@@ -63,7 +63,7 @@ constexpr int SORT_BITS = 9, SORT_BINS = 1 << SORT_BITS, SORT_TILE = 2048, SORT_
 __device__ __forceinline__ unsigned sort_key(long long id, unsigned vocab) { return id >= 0 && id < (long long)vocab ? (unsigned)id : vocab; }
 
 // Short lists (n <= RANK_MAX): a token's place is the number of smaller keys plus the number of equal keys in front of it, counted against all keys in LDS.
-// 64 tokens per block, its 16 waves count a sixteenth of the list each.  n^2 / 2 comparisons, two instructions each, on all CUs - and one launch.
+// 64 tokens per block, its 16 waves count a sixteenth of the list each.  n^2 comparisons, two instructions each, on n / 64 blocks - and one launch.
 // Added to a table (us, with the sums; ids spread / all equal) against the radix passes: 500 tokens 17 / 15 against 30 / 28, 5 000: 36 / 29 against 49 / 43,
 // 15 360: 83 / 72 against 86 / 75 - about equal where the keys fill 60 KiB.
 constexpr int RANK_MAX = 15360, RANK_WAVES = 16;
