@@ -311,9 +311,9 @@ int vitg_embed_backward(const long long* ids, long n, const void* dout, int dout
  * vitg_swiglu: as vitg_gemm(mode = VITG_GEMM_SWIGLU); with gu != NULL it also stores [G | U] rounded to `dtype` in the weight rows' order ([M, N]) for the
  *   backward pass.  K % 64 == 0, N % 64 == 0, leading dimensions multiples of 8, 16-byte aligned pointers.
  * vitg_swiglu_backward: from dout = dL/d out and the saved gu: dX = dGU W (type dtype, overwritten) and dW (+)= dGU^T X (type dtype or fp32; accumulate = 1
- *   adds to what it holds), dGU rounded to dtype once - the matrix pipe's operand type; an fp16
- *   value beyond 65 504 becomes infinite and one below 2^-25 zero, as in fp16 autograd: scale the loss for it; either of dX / dW may be NULL (then W / X is not read).  workspace: vitg_swiglu_backward_plan bytes,
- *   16-byte aligned.  M = 0: dW becomes zero (accumulate = 0) or stays. */
+ *   adds to what it holds), dGU rounded to dtype once - the matrix pipe's operand type (an fp16 value beyond 65 504 becomes infinite, one below 2^-25 zero, as in
+ *   fp16 autograd: scale the loss for it); either of dX / dW may be NULL (then W / X is not read).  workspace: vitg_swiglu_backward_plan bytes, 16-byte
+ *   aligned.  M = 0: dW becomes zero (accumulate = 0) or stays. */
 int vitg_swiglu(const void* X, int ldx, const void* W, int ldw, int M, int N, int K, int dtype, void* out, int ldo, void* gu, int ldgu, void* stream);
 int vitg_swiglu_backward_plan(int M, int N, int K, int want_dx, int want_dw, long* workspace_bytes);
 int vitg_swiglu_backward(const void* dout, int lddo, const void* gu, int ldgu, const void* X, int ldx, const void* W, int ldw, int M, int N, int K, int dtype,
