@@ -90,6 +90,10 @@ def test_dispatcher_form_of_clipping_takes_every_argument(ops):
     zeros = lambda: [torch.zeros_like(t) for t in make()]                                                     # noqa: E731
     with pytest.raises(Exception, match="no outs"):
         K.clip_grad_norm(make(), None, outs=zeros())
+    with pytest.raises(Exception, match="no outs"):
+        torch.ops.videoitg.clip_grad_norm_into(make(), zeros(), torch.zeros(1, device="cuda"), None)
+    with pytest.raises(Exception, match="2 gradients and 0 outputs"):
+        torch.ops.videoitg.clip_grad_norm_into(make(), [], torch.zeros(1, device="cuda"), 1.0)
     ws = torch.empty(4096, dtype=torch.uint8, device="cuda")
     for max_norm in (0.5, None):
         for outs in (False, True):

@@ -218,7 +218,7 @@ _def("clip_grad_norm_(Tensor(a!)[] grads, float max_norm, float scale=1.0) -> Te
 
 _def("clip_grad_norm_into(Tensor[] grads, Tensor(a!)[] outs, Tensor(b!) norm, float? max_norm, float scale=1.0, Tensor(c!)? workspace=None) -> ()",
      lambda grads, outs, norm, max_norm, scale=1.0, workspace=None:
-         (_raw.clip_grad_norm(grads, max_norm, outs=None if max_norm is None else outs, scale=scale, norm=norm, workspace=workspace), None)[1],
+         (_raw.clip_grad_norm(grads, max_norm, outs=outs if outs or max_norm is not None else None, scale=scale, norm=norm, workspace=workspace), None)[1],
      lambda *a, **k: None)
 
 # ---- call-compatible namespace for the engine (same signatures as videoitg_amd.ops) ------------------------------------
